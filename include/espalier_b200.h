@@ -325,6 +325,101 @@ int esp_ep_out(const float* y, const int* local_pick, int world, int rank, int R
                int D, float* const* inbox_y, int* const* flags_y, const int* pick, const float* wts, void* out,
                void* out_shared, int out_dtype, int* epoch, int* done, int* count, int returned, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Around the coded projections of a decode step: the norms and residual add between two blocks, low-rank adapters
+ * beside a projection, and the verification of drafted tokens. No counterpart in the reference.
+ * --------------------------------------------------------------------------------------------------------------- */
+
+/* normalisation */
+#define ESP_NORM_NONE 0
+#define ESP_NORM_RMS 1   /* v / sqrt(mean(v^2) + eps) */
+#define ESP_NORM_LAYER 2 /* (v - mean) / sqrt(mean((v - mean)^2) + eps) */
+
+/* gate shape and activation */
+#define ESP_GATE_NONE 0
+#define ESP_GATE_CHANNEL 1 /* [d], the same for every row */
+#define ESP_GATE_ROW 2     /* one value a row, `gate_stride` elements apart */
+#define ESP_GATE_ELEMENT 3 /* [rows][d] */
+#define ESP_ACT_NONE 0
+#define ESP_ACT_SIGMOID 1
+#define ESP_ACT_TANH 2
+
+/* What a block norm keeps between calls. Weights and biases: [d] of w_dtype, contiguous, or NULL (ones / zeros). */
+typedef struct esp_block_norm_op {
+    int d;                  /* columns, 1 .. 49152 */
+    int post, pre;          /* ESP_NORM_*: the norm of the block's output, the norm before the next block */
+    int gate_act;           /* ESP_ACT_* */
+    float eps, weight_offset; /* a norm multiplies by weight_offset + weight */
+    float residual_scale, block_scale;
+    int w_dtype;
+    const void *post_w, *post_b, *pre_w, *pre_b;
+} esp_block_norm_op_t;
+
+/*
+ * Between two blocks, for each of `rows` rows:
+ *   v = x (+ x2);  p = post(v);  r = residual_scale * residual + block_scale * act(gate) * p;  h = pre(r)
+ * r goes to r_out in r_dtype and h to h_out in x_dtype. x2, residual and the gate may be NULL (no term; no factor),
+ * r_out may be NULL (not stored), h_out is NULL exactly when op->pre is ESP_NORM_NONE. Everything is computed in fp32
+ * from the inputs and rounded once per output: h is the norm of the unrounded r. x and x2 share x_dtype, residual and
+ * r_out r_dtype; the row strides are in elements. r_out may be residual or x itself, h_out x itself (same stride);
+ * no other overlap. A row's bits do not depend on the other rows.
+ */
+int esp_block_norm(const esp_block_norm_op_t* op, const void* x, long long x_stride, const void* x2,
+                   long long x2_stride, int x_dtype, const void* residual, long long residual_stride, int r_dtype,
+                   const void* gate, int gate_kind, int gate_dtype, long long gate_stride, void* r_out,
+                   long long r_out_stride, void* h_out, long long h_out_stride, long long rows, void* stream);
+
+/*
+ * Low-rank adapters of up to `slots` requests' kinds beside one projection of n_mats matrices (q | k | v side by side).
+ * All arrays are device memory, contiguous and 16-byte aligned, a and b of the rows' dtype:
+ *   a      [slots][n_mats][rank][k]       ranks  int32 [slots], or NULL: every slot has the full rank
+ *   b      [slots][sum(widths)][rank]     scales fp32 [slots], or NULL: ones
+ * rank is the capacity, a multiple of 8 up to 128; k and every width are multiples of 8; at most 4096 slots. A slot of rank q reads the
+ * rows of a and the columns of b below q rounded up to 8 (those from q on hold zeros) and nothing past them.
+ */
+typedef struct esp_adapters {
+    const void *a, *b;
+    const int* ranks;
+    const float* scales;
+    int dtype; /* ESP_DTYPE_F16 or ESP_DTYPE_BF16: a, b and the rows */
+    int slots, rank, k, n_mats;
+    int widths[4];
+} esp_adapters_t;
+
+/*
+ * out[t] = y[t] + scales[a] * (x[t] A[a, s]^T) B[a, s]^T for every matrix s, a = ids[t] (int32 [t_rows]); a row whose
+ * id is outside [0, slots), or whose slot has rank 0, gets y[t]. x [t_rows][k], y and out [t_rows][sum(widths)] in
+ * the adapters' dtype, rows 16-byte aligned (strides in elements, multiples of 8); out may be y itself. The inner
+ * product is held in fp32 and the sum rounded once. A row's bits depend on its own id, x and y only.
+ * ws: esp_adapt_ws_bytes(t_rows, slots) bytes of device memory, 16-byte aligned, of any content (NULL when that is 0).
+ */
+int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_stride, const void* y, long long y_stride,
+              const int* ids, int t_rows, void* out, long long out_stride, void* ws, size_t ws_bytes, void* stream);
+size_t esp_adapt_ws_bytes(int t_rows, int slots);
+
+/*
+ * Verification of drafted tokens. Request b of `requests` has k_b = starts[b + 1] - starts[b] drafted tokens (starts
+ * int32 [requests + 1], ascending from 0) and k_b + 1 rows of target logits: rows starts[b] + b .. starts[b] + b + k_b
+ * of logits [rows][vocab], row i the target's logits for the place of its i-th drafted token, the last row for the
+ * place after them. With p_i = softmax(row i / temperature[b]) and q_i the drafter's probabilities (draft_probs
+ * [n_drafts][vocab]; NULL: the drafter chose its token with probability one):
+ *   drafted token d_i stands iff all before it do and uniform[i] * q_i(d_i) < p_i(d_i), uniform in [0, 1);
+ *   the first that falls is replaced by argmax_v max(p_i(v) - q_i(v), 0) / noise[b][v]; if all stand, one more token is
+ *   argmax_v p(v) / noise[b][v] of the last row (noise: independent exponential numbers, so these are draws from the
+ *   residual and the target; ties to the lowest id; the target's likeliest token where the residual is zero).
+ * A temperature that is not above 0 is greedy: d_i stands iff it is the argmax, which replaces it otherwise.
+ * tokens int32 [requests][max_drafts + 1] gets the tokens that stand and the drawn one, -1 after them; accepted int32
+ * [requests] the number that stand; probs fp32 [requests][max_drafts + 1] p_i of each token (temperature 1 for a greedy
+ * request), 0 after them. NaN logits count as -inf (a token ruled out); a row with nothing left gives -1 and ends the
+ * request. A drafted id outside [0, vocab) never stands. Drafts past max_drafts are not looked at; a request whose
+ * starts do not fit rows and n_drafts gets no token. Strides in elements; temperature NULL: 1, and one outside
+ * [1e-30, 1e30] counts as the nearer end.
+ */
+int esp_verify(const void* logits, int dtype, long long stride, long long rows, int vocab, const int* starts,
+               int requests, const int* drafts, const float* uniform, long long n_drafts, const void* draft_probs,
+               int probs_dtype, long long probs_stride, const float* noise, long long noise_stride,
+               const float* temperature, int max_drafts, int* tokens, int* accepted, float* probs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,6 +34,19 @@ class esp_matrix_t(C.Structure):
                 ("col0", C.c_int)]
 
 
+class esp_block_norm_op_t(C.Structure):
+    _fields_ = [("d", C.c_int), ("post", C.c_int), ("pre", C.c_int), ("gate_act", C.c_int), ("eps", C.c_float),
+                ("weight_offset", C.c_float), ("residual_scale", C.c_float), ("block_scale", C.c_float),
+                ("w_dtype", C.c_int), ("post_w", C.c_void_p), ("post_b", C.c_void_p), ("pre_w", C.c_void_p),
+                ("pre_b", C.c_void_p)]
+
+
+class esp_adapters_t(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("ranks", C.c_void_p), ("scales", C.c_void_p),
+                ("dtype", C.c_int), ("slots", C.c_int), ("rank", C.c_int), ("k", C.c_int), ("n_mats", C.c_int),
+                ("widths", C.c_int * 4)]
+
+
 P, I, L, S, F = C.c_void_p, C.c_int, C.c_longlong, C.c_size_t, C.c_float
 SIGNATURES = {
     "esp_version": (I, []),
@@ -71,6 +84,10 @@ SIGNATURES = {
                       P, P, P, P, P]),
     "esp_moe_layer_ep": (I, [P, P, P, P, P, P, P, P, P, P, P, P, P, I, P, P, P, P, P, P, P, I, I, P, P, I, I, I, I, I,
                              P, P, P, C.POINTER(P), C.POINTER(P), P, I, I, I, P, P]),
+    "esp_block_norm": (I, [P, P, L, P, L, I, P, L, I, P, I, I, L, P, L, P, L, L, P]),
+    "esp_adapt": (I, [P, P, L, P, L, P, I, P, L, P, S, P]),
+    "esp_adapt_ws_bytes": (S, [I, I]),
+    "esp_verify": (I, [P, I, L, L, I, P, I, P, P, L, P, I, L, P, L, P, I, P, P, P, P]),
     "esp_ep_out": (I, [P, P, I, I, I, I, I, I, I, C.POINTER(P), C.POINTER(P), P, P, P, P, I, P, P, P, I, P]),
 }
 
