@@ -3,6 +3,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "host.hpp"
 
@@ -66,7 +68,7 @@ __device__ __forceinline__ float affine(float v, const NormParams& p, const void
     return b ? v + load1(b, p.op.w_dtype, i) : v;
 }
 
-// Any width, alignment and type: a CTA a row, the row in shared memory as fp32.
+// Any width, alignment and mix of types: a CTA a row, the row in shared memory as fp32.
 __global__ void block_norm_kernel(NormParams p) {
     extern __shared__ float row[];
     __shared__ float scratch[32];
@@ -100,8 +102,253 @@ __global__ void block_norm_kernel(NormParams p) {
         store1(p.h_out, p.x_dtype, t * p.h_out_stride + i, affine((row[i] - mean) * inv, p, p.op.pre_w, p.op.pre_b, i));
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// The row in registers: thread i of NT holds VPT groups of VEC consecutive columns, group j at column (j NT + i) VEC.
+// Every input of the row is asked for before the first sum, so a row costs one memory round trip, its reductions (one
+// barrier each) and the stores. VEC 8: 16-byte loads, the weights asked for with the rest; VEC 1: any width and
+// alignment, a register a value, so the weights (and always the biases) are read where they are used.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T) >= 16 ? 16 : sizeof(T)) Group {
+    T e[VEC];
+};
+
+__device__ __forceinline__ float f32(float v) { return v; }
+__device__ __forceinline__ float f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// A group rounded to its type, two values an instruction where there are two.
+template <int VEC>
+__device__ __forceinline__ void rounded(const float (&v)[VEC], Group<float, VEC>& g) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) g.e[e] = v[e];
+}
+template <int VEC>
+__device__ __forceinline__ void rounded(const float (&v)[VEC], Group<__half, VEC>& g) {
+    if constexpr (VEC == 1) g.e[0] = __float2half_rn(v[0]);
+    else
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) *reinterpret_cast<__half2*>(&g.e[e]) = __floats2half2_rn(v[e], v[e + 1]);
+}
+template <int VEC>
+__device__ __forceinline__ void rounded(const float (&v)[VEC], Group<__nv_bfloat16, VEC>& g) {
+    if constexpr (VEC == 1) g.e[0] = __float2bfloat16_rn(v[0]);
+    else
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2)
+            *reinterpret_cast<__nv_bfloat162*>(&g.e[e]) = __floats2bfloat162_rn(v[e], v[e + 1]);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void fetch(Group<T, VEC>& g, const void* base, size_t i) {
+    g = *reinterpret_cast<const Group<T, VEC>*>(static_cast<const T*>(base) + i);
+}
+
+// The sum over the CTA with one barrier; `scratch` (a word a warp) is this reduction's own.
+template <int NT>
+__device__ __forceinline__ float rows_sum(float v, float* scratch) {
+#pragma unroll
+    for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) s += scratch[w];
+    return s;
+}
+
+// v becomes (v - mean) for a layer norm; inv the reciprocal root of its second moment. Columns past d hold 0 in v.
+template <int NT, int VEC, int VPT>
+__device__ __forceinline__ float rows_moments(float (&v)[VPT][VEC], int d, int kind, float eps, float (*scratch)[32]) {
+    if (kind == ESP_NORM_LAYER) {
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s += v[j][e];
+        const float mean = rows_sum<NT>(s, scratch[0]) / d;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+            if ((j * NT + static_cast<int>(threadIdx.x)) * VEC < d)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[j][e] -= mean;
+    }
+    float q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) q = fmaf(v[j][e], v[j][e], q);
+    return rsqrtf(rows_sum<NT>(q, scratch[1]) / d + eps);
+}
+
+template <typename TX, typename TR, typename TW, int VEC, int NT, int VPT>
+__global__ void __launch_bounds__(NT) block_norm_rows(NormParams p) {
+    __shared__ float scratch[4][32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const size_t t = blockIdx.x;
+    const int d = p.op.d;
+    const bool gated = p.gate_kind == ESP_GATE_ELEMENT || p.gate_kind == ESP_GATE_CHANNEL;
+    const size_t gate_at = p.gate_kind == ESP_GATE_ELEMENT ? t * p.gate_stride : 0;
+    Group<TX, VEC> x[VPT], x2[VPT], gate[VPT];
+    Group<TR, VEC> res[VPT];
+    Group<TW, VEC> post_w[VPT], pre_w[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int c = (j * NT + static_cast<int>(threadIdx.x)) * VEC;
+        if (c >= d) continue;
+        fetch(x[j], p.x, t * p.x_stride + c);
+        if (p.x2) fetch(x2[j], p.x2, t * p.x2_stride + c);
+        if (p.residual) fetch(res[j], p.residual, t * p.residual_stride + c);
+        if (gated) fetch(gate[j], p.gate, gate_at + c);
+        if (VEC > 1 && p.op.post_w) fetch(post_w[j], p.op.post_w, c);
+        if (VEC > 1 && p.op.pre_w) fetch(pre_w[j], p.op.pre_w, c);
+    }
+    float scale = p.op.block_scale;
+    if (p.gate_kind == ESP_GATE_ROW) scale *= activation(load1(p.gate, p.gate_dtype, t * p.gate_stride), p.op.gate_act);
+
+    float v[VPT][VEC];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const bool in = (j * NT + static_cast<int>(threadIdx.x)) * VEC < d;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[j][e] = in ? f32(x[j].e[e]) : 0.0f;
+        if (in && p.x2)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[j][e] += f32(x2[j].e[e]);
+    }
+    // Each term a branch of the whole group, not of each value.
+    const float inv = p.op.post ? rows_moments<NT, VEC, VPT>(v, d, p.op.post, p.op.eps, scratch) : 1.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int c = (j * NT + static_cast<int>(threadIdx.x)) * VEC;
+        if (c >= d) continue;
+        float(&a)[VEC] = v[j];
+        if (p.op.post)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[e] *= inv;
+        if (p.op.post_w) {
+            if (VEC == 1) fetch(post_w[j], p.op.post_w, c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[e] *= p.op.weight_offset + f32(post_w[j].e[e]);
+        }
+        if (p.op.post_b) {
+            Group<TW, VEC> b;
+            fetch(b, p.op.post_b, c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[e] += f32(b.e[e]);
+        }
+        if (gated) {
+            float g[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) g[e] = f32(gate[j].e[e]);
+            if (p.op.gate_act != ESP_ACT_NONE)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) g[e] = activation(g[e], p.op.gate_act);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[e] *= g[e];
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) a[e] *= scale;
+        if (p.residual)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[e] = fmaf(p.op.residual_scale, f32(res[j].e[e]), a[e]);
+        if (p.r_out) {
+            Group<TR, VEC> r;
+            rounded(a, r);
+            *reinterpret_cast<Group<TR, VEC>*>(static_cast<TR*>(p.r_out) + t * p.r_out_stride + c) = r;
+        }
+    }
+    if (!p.op.pre) return;
+    const float inv2 = rows_moments<NT, VEC, VPT>(v, d, p.op.pre, p.op.eps, scratch + 2);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int c = (j * NT + static_cast<int>(threadIdx.x)) * VEC;
+        if (c >= d) continue;
+        float(&a)[VEC] = v[j];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) a[e] *= inv2;
+        if (p.op.pre_w) {
+            if (VEC == 1) fetch(pre_w[j], p.op.pre_w, c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[e] *= p.op.weight_offset + f32(pre_w[j].e[e]);
+        }
+        if (p.op.pre_b) {
+            Group<TW, VEC> b;
+            fetch(b, p.op.pre_b, c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[e] += f32(b.e[e]);
+        }
+        Group<TX, VEC> h;
+        rounded(a, h);
+        *reinterpret_cast<Group<TX, VEC>*>(static_cast<TX*>(p.h_out) + t * p.h_out_stride + c) = h;
+    }
+}
+
 constexpr int MAX_D = 49152;   // the row as fp32 in shared memory: 192 KB
 bool known_dtype(int t) { return t == F16 || t == BF16 || t == F32; }
+
+// Whether every row of a tensor starts on a 16-byte boundary (NULL: nothing to load).
+bool vector_rows(const void* p, int dtype, long long stride) {
+    return !p || (aligned(p, 16) && stride % (dtype == F32 ? 4 : 8) == 0);
+}
+
+struct RowsKernel {
+    void (*run)(NormParams) = nullptr;
+    int threads = 0;
+};
+
+template <typename TX, typename TR, typename TW, int VEC, int NT, int VPT>
+RowsKernel rows_instance() {
+    return {block_norm_rows<TX, TR, TW, VEC, NT, VPT>, NT};
+}
+
+// The registers' kernel for this width, none where the row does not fit: the threads a row needs for one group each
+// (two at most), so that a row's order of summation depends on its width and whether vector loads fit, not on the
+// number of rows.
+template <typename TX, typename TR, typename TW>
+RowsKernel rows_kernel(int d, bool vec) {
+    if (vec) {
+        if (d <= 1024) return rows_instance<TX, TR, TW, 8, 128, 1>();
+        if (d <= 2048) return rows_instance<TX, TR, TW, 8, 256, 1>();
+        if (d <= 4096) return rows_instance<TX, TR, TW, 8, 512, 1>();
+        if (d <= 8192) return rows_instance<TX, TR, TW, 8, 512, 2>();
+        return {};
+    }
+    if (d <= 2048) return rows_instance<TX, TR, TW, 1, 256, 8>();
+    if (d <= 8192) return rows_instance<TX, TR, TW, 1, 1024, 8>();
+    return {};
+}
+
+template <typename TX>
+RowsKernel rows_kernel(const NormParams& p, bool vec) {
+    const bool r32 = p.r_dtype == F32, w32 = p.op.w_dtype == F32;
+    if (r32 && w32) return rows_kernel<TX, float, float>(p.op.d, vec);
+    if constexpr (!std::is_same_v<TX, float>) {
+        if (r32) return rows_kernel<TX, float, TX>(p.op.d, vec);
+        if (w32) return rows_kernel<TX, TX, float>(p.op.d, vec);
+        return rows_kernel<TX, TX, TX>(p.op.d, vec);
+    }
+    return {};
+}
+
+// The kernel for a call: the registers' one where its types are those a model mixes (x's own or fp32 for the stream and
+// for the weights, x's own for a gate of more than a value a row), none otherwise.
+RowsKernel rows_kernel(const NormParams& p) {
+    const auto fits = [&](int dtype) { return dtype == p.x_dtype || dtype == F32; };
+    const bool gated = p.gate_kind == ESP_GATE_CHANNEL || p.gate_kind == ESP_GATE_ELEMENT;
+    if (!fits(p.r_dtype) || !fits(p.op.w_dtype) || (gated && p.gate_dtype != p.x_dtype)) return {};
+    const bool vec = p.op.d % 8 == 0 && vector_rows(p.x, p.x_dtype, p.x_stride) &&
+                     vector_rows(p.x2, p.x_dtype, p.x2_stride) &&
+                     vector_rows(p.residual, p.r_dtype, p.residual_stride) &&
+                     (!gated || vector_rows(p.gate, p.gate_dtype, p.gate_kind == ESP_GATE_ELEMENT ? p.gate_stride : 0)) &&
+                     vector_rows(p.r_out, p.r_dtype, p.r_out_stride) && vector_rows(p.h_out, p.x_dtype, p.h_out_stride) &&
+                     vector_rows(p.op.post_w, p.op.w_dtype, 0) && vector_rows(p.op.post_b, p.op.w_dtype, 0) &&
+                     vector_rows(p.op.pre_w, p.op.w_dtype, 0) && vector_rows(p.op.pre_b, p.op.w_dtype, 0);
+    if (p.x_dtype == BF16) return rows_kernel<__nv_bfloat16>(p, vec);
+    if (p.x_dtype == F16) return rows_kernel<__half>(p, vec);
+    return rows_kernel<float>(p, vec);
+}
 
 }  // namespace
 }  // namespace esp
@@ -133,6 +380,10 @@ extern "C" int esp_block_norm(const esp_block_norm_op_t* op, const void* x, long
     ESP_REQUIRE(r_out || h_out, ESP_ERR_INVALID, "esp_block_norm: no output");
     NormParams p{*op, x, x2, residual, gate, r_out, h_out, x_stride, x2_stride, residual_stride, gate_stride,
                  r_out_stride, h_out_stride, x_dtype, r_dtype, gate_kind, gate_dtype};
+    if (const RowsKernel k = rows_kernel(p); k.run) {
+        if (const int rc = launch(k.run, dim3(static_cast<unsigned>(rows)), dim3(k.threads), 0, stream, true, p)) return rc;
+        return ok();
+    }
     const size_t smem = static_cast<size_t>(op->d) * 4;
     if (const int rc = allow_smem(block_norm_kernel, smem)) return rc;
     if (const int rc = launch(block_norm_kernel, dim3(static_cast<unsigned>(rows)), dim3(op->d <= 4096 ? 256 : 1024), smem,
