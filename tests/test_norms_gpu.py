@@ -120,6 +120,20 @@ def test_many_rows(dev, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d,rows", [(8, 5000), (256, 2500), (1000, 1300), (1408, 1500), (4096, 500), (8192, 400)])
+@pytest.mark.parametrize("kind,gate,act", [("rms", "element", "sigmoid"), ("layer", "channel", "tanh")])
+def test_many_rows_of_other_widths(dev, d, rows, kind, gate, act):
+    """More rows than the GPU takes at once, and a row alone: the same bits."""
+    dtype, r_dtype = DT[d // 8 % 4]
+    op, t, r, h = run_and_check(dev, rows, d, dtype, r_dtype, kind, two=d != 1000, gate=gate, act=act, seed=d)
+    for i in (0, rows // 2, rows - 1):
+        one = slice(i, i + 1)
+        r1, h1 = op(t["x"][one], t["residual"][one], x2=None if t["x2"] is None else t["x2"][one],
+                    gate=t["gate"] if gate == "channel" else t["gate"][one])
+        assert torch.equal(r1, r[one]) and torch.equal(h1, h[one])
+
+
+@pytest.mark.gpu
 def test_weight_offset(dev):
     run_and_check(dev, 9, 2048, torch.bfloat16, torch.bfloat16, offset=1.0)
 

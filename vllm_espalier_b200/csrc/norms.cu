@@ -3,6 +3,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -31,8 +32,10 @@ __device__ __forceinline__ void store1(void* p, int dtype, size_t i, float v) {
     else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// The fast exponential and division: within 4 units of fp32 plus |g| units for the exponential's scaled argument, far
+// inside every output's rounding, and a third of the exact ones' instructions, which a gate a value pays per value.
 __device__ __forceinline__ float activation(float g, int act) {
-    if (act == ESP_ACT_SIGMOID) return 1.0f / (1.0f + expf(-g));
+    if (act == ESP_ACT_SIGMOID) return __fdividef(1.0f, 1.0f + __expf(-g));
     if (act == ESP_ACT_TANH) return tanhf(g);
     return g;
 }
@@ -149,12 +152,16 @@ template <int NT>
 __device__ __forceinline__ float rows_sum(float v, float* scratch) {
 #pragma unroll
     for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    if (NT == 32) return v;
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
     __syncthreads();
-    float s = 0.0f;
+    float4 s = *reinterpret_cast<const float4*>(scratch);       // NT is a multiple of 128
 #pragma unroll
-    for (int w = 0; w < NT / 32; ++w) s += scratch[w];
-    return s;
+    for (int w = 4; w < NT / 32; w += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(scratch + w);
+        s.x += u.x, s.y += u.y, s.z += u.z, s.w += u.w;
+    }
+    return (s.x + s.y) + (s.z + s.w);
 }
 
 // v becomes (v - mean) for a layer norm; inv the reciprocal root of its second moment. Columns past d hold 0 in v.
@@ -181,43 +188,85 @@ __device__ __forceinline__ float rows_moments(float (&v)[VPT][VEC], int d, int k
     return rsqrtf(rows_sum<NT>(q, scratch[1]) / d + eps);
 }
 
-template <typename TX, typename TR, typename TW, int VEC, int NT, int VPT>
-__global__ void __launch_bounds__(NT) block_norm_rows(NormParams p) {
-    __shared__ float scratch[4][32];
-    pdl_launch_dependents();
-    pdl_wait();
-    const size_t t = blockIdx.x;
-    const int d = p.op.d;
-    const bool gated = p.gate_kind == ESP_GATE_ELEMENT || p.gate_kind == ESP_GATE_CHANNEL;
-    const size_t gate_at = p.gate_kind == ESP_GATE_ELEMENT ? t * p.gate_stride : 0;
-    Group<TX, VEC> x[VPT], x2[VPT], gate[VPT];
-    Group<TR, VEC> res[VPT];
+// A row's inputs as a thread gets at them, group j at column c: held in registers, or read where they are used out of a
+// stage of shared memory (x, x2, gate, residual one after another).
+template <typename TX, typename TR, int VEC, int VPT>
+struct InRegisters {
+    Group<TX, VEC> x_[VPT], x2_[VPT], gate_[VPT];
+    Group<TR, VEC> res_[VPT];
+    __device__ __forceinline__ Group<TX, VEC> x(int j, int) const { return x_[j]; }
+    __device__ __forceinline__ Group<TX, VEC> x2(int j, int) const { return x2_[j]; }
+    __device__ __forceinline__ Group<TX, VEC> gate(int j, int) const { return gate_[j]; }
+    __device__ __forceinline__ Group<TR, VEC> res(int j, int) const { return res_[j]; }
+};
+template <typename TX, typename TR, int VEC>
+struct InStage {
+    const unsigned char *x_, *x2_, *gate_, *res_;     // gate_: a row's, or the channels' in global memory
+    template <typename T>
+    static __device__ __forceinline__ Group<T, VEC> get(const unsigned char* p, int c) {
+        return *reinterpret_cast<const Group<T, VEC>*>(p + c * sizeof(T));
+    }
+    __device__ __forceinline__ Group<TX, VEC> x(int, int c) const { return get<TX>(x_, c); }
+    __device__ __forceinline__ Group<TX, VEC> x2(int, int c) const { return get<TX>(x2_, c); }
+    __device__ __forceinline__ Group<TX, VEC> gate(int, int c) const { return get<TX>(gate_, c); }
+    __device__ __forceinline__ Group<TR, VEC> res(int, int c) const { return get<TR>(res_, c); }
+};
+template <typename TW, int VEC, int VPT>
+struct RowWeights {
     Group<TW, VEC> post_w[VPT], pre_w[VPT];
+};
+
+__device__ __forceinline__ bool gated(const NormParams& p) {
+    return p.gate_kind == ESP_GATE_ELEMENT || p.gate_kind == ESP_GATE_CHANNEL;
+}
+
+template <typename TW, int VEC>
+__device__ __forceinline__ void scale_by(float (&a)[VEC], const Group<TW, VEC>& w, float offset) {
+    if (offset != 0.0f) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) a[e] *= offset + f32(w.e[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) a[e] *= f32(w.e[e]);
+    }
+}
+
+template <typename TW, int VEC, int NT, int VPT>
+__device__ __forceinline__ void fetch_weights(RowWeights<TW, VEC, VPT>& w, const NormParams& p) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int c = (j * NT + static_cast<int>(threadIdx.x)) * VEC;
-        if (c >= d) continue;
-        fetch(x[j], p.x, t * p.x_stride + c);
-        if (p.x2) fetch(x2[j], p.x2, t * p.x2_stride + c);
-        if (p.residual) fetch(res[j], p.residual, t * p.residual_stride + c);
-        if (gated) fetch(gate[j], p.gate, gate_at + c);
-        if (VEC > 1 && p.op.post_w) fetch(post_w[j], p.op.post_w, c);
-        if (VEC > 1 && p.op.pre_w) fetch(pre_w[j], p.op.pre_w, c);
+        if (c < p.op.d && p.op.post_w) fetch(w.post_w[j], p.op.post_w, c);
+        if (c < p.op.d && p.op.pre_w) fetch(w.pre_w[j], p.op.pre_w, c);
     }
+}
+
+// Row t from its inputs to its outputs. Each term is a branch of the whole group, not of each value. WEIGHTS: the weights
+// are in `w`, otherwise they are read where they are used.
+template <typename TX, typename TR, typename TW, int VEC, int NT, int VPT, bool WEIGHTS, typename In>
+__device__ __forceinline__ void norm_row(const NormParams& p, size_t t, const In& in, RowWeights<TW, VEC, VPT>& w,
+                                         float (*scratch)[32]) {
+    const int d = p.op.d;
     float scale = p.op.block_scale;
     if (p.gate_kind == ESP_GATE_ROW) scale *= activation(load1(p.gate, p.gate_dtype, t * p.gate_stride), p.op.gate_act);
-
     float v[VPT][VEC];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        const bool in = (j * NT + static_cast<int>(threadIdx.x)) * VEC < d;
+        const int c = (j * NT + static_cast<int>(threadIdx.x)) * VEC;
+        if (c < d) {
+            const Group<TX, VEC> x = in.x(j, c);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[j][e] = in ? f32(x[j].e[e]) : 0.0f;
-        if (in && p.x2)
+            for (int e = 0; e < VEC; ++e) v[j][e] = f32(x.e[e]);
+            if (p.x2) {
+                const Group<TX, VEC> x2 = in.x2(j, c);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[j][e] += f32(x2[j].e[e]);
+                for (int e = 0; e < VEC; ++e) v[j][e] += f32(x2.e[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[j][e] = 0.0f;
+        }
     }
-    // Each term a branch of the whole group, not of each value.
     const float inv = p.op.post ? rows_moments<NT, VEC, VPT>(v, d, p.op.post, p.op.eps, scratch) : 1.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
@@ -228,9 +277,8 @@ __global__ void __launch_bounds__(NT) block_norm_rows(NormParams p) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) a[e] *= inv;
         if (p.op.post_w) {
-            if (VEC == 1) fetch(post_w[j], p.op.post_w, c);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) a[e] *= p.op.weight_offset + f32(post_w[j].e[e]);
+            if (!WEIGHTS) fetch(w.post_w[j], p.op.post_w, c);
+            scale_by(a, w.post_w[j], p.op.weight_offset);
         }
         if (p.op.post_b) {
             Group<TW, VEC> b;
@@ -238,10 +286,11 @@ __global__ void __launch_bounds__(NT) block_norm_rows(NormParams p) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) a[e] += f32(b.e[e]);
         }
-        if (gated) {
+        if (gated(p)) {
+            const Group<TX, VEC> gate = in.gate(j, c);
             float g[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) g[e] = f32(gate[j].e[e]);
+            for (int e = 0; e < VEC; ++e) g[e] = f32(gate.e[e]);
             if (p.op.gate_act != ESP_ACT_NONE)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) g[e] = activation(g[e], p.op.gate_act);
@@ -250,9 +299,11 @@ __global__ void __launch_bounds__(NT) block_norm_rows(NormParams p) {
         }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) a[e] *= scale;
-        if (p.residual)
+        if (p.residual) {
+            const Group<TR, VEC> res = in.res(j, c);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) a[e] = fmaf(p.op.residual_scale, f32(res[j].e[e]), a[e]);
+            for (int e = 0; e < VEC; ++e) a[e] = fmaf(p.op.residual_scale, f32(res.e[e]), a[e]);
+        }
         if (p.r_out) {
             Group<TR, VEC> r;
             rounded(a, r);
@@ -269,9 +320,8 @@ __global__ void __launch_bounds__(NT) block_norm_rows(NormParams p) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) a[e] *= inv2;
         if (p.op.pre_w) {
-            if (VEC == 1) fetch(pre_w[j], p.op.pre_w, c);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) a[e] *= p.op.weight_offset + f32(pre_w[j].e[e]);
+            if (!WEIGHTS) fetch(w.pre_w[j], p.op.pre_w, c);
+            scale_by(a, w.pre_w[j], p.op.weight_offset);
         }
         if (p.op.pre_b) {
             Group<TW, VEC> b;
@@ -285,6 +335,95 @@ __global__ void __launch_bounds__(NT) block_norm_rows(NormParams p) {
     }
 }
 
+template <typename TX, typename TR, typename TW, int VEC, int NT, int VPT>
+__global__ void __launch_bounds__(NT) block_norm_rows(NormParams p) {
+    __shared__ __align__(16) float scratch[4][32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const size_t t = blockIdx.x;
+    InRegisters<TX, TR, VEC, VPT> in;
+    RowWeights<TW, VEC, VPT> w;
+    const size_t gate_at = p.gate_kind == ESP_GATE_ELEMENT ? t * p.gate_stride : 0;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int c = (j * NT + static_cast<int>(threadIdx.x)) * VEC;
+        if (c >= p.op.d) continue;
+        fetch(in.x_[j], p.x, t * p.x_stride + c);
+        if (p.x2) fetch(in.x2_[j], p.x2, t * p.x2_stride + c);
+        if (p.residual) fetch(in.res_[j], p.residual, t * p.residual_stride + c);
+        if (gated(p)) fetch(in.gate_[j], p.gate, gate_at + c);
+    }
+    if constexpr (VEC > 1) fetch_weights<TW, VEC, NT, VPT>(w, p);
+    norm_row<TX, TR, TW, VEC, NT, VPT, (VEC > 1)>(p, t, in, w, scratch);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Many rows: a CTA walks its rows (blockIdx, + gridDim, ...), the next STAGES rows' inputs on their way into a ring of
+// shared memory by bulk copies (one thread asks, an mbarrier a stage counts the bytes), so the copies in flight do not
+// depend on how many registers the threads hold, and the weights stay in registers over the rows. Same columns a
+// thread and same sums as block_norm_rows, so the same bits.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int MAX_STAGES = 8;
+constexpr int RING_BYTES = 227 * 1024;          // an SM's shared memory for its CTAs' rings
+constexpr int RING_FIXED = 4 * 1024;            // of it, a CTA's barriers, scratch and the 1 KB the system keeps, rounded up
+// CTAs an SM: 1024 threads of them at 64 registers each (a thread with two groups needs twice that).
+constexpr int ring_ctas(int threads, int groups) { return groups > 1 ? 1 : threads >= 64 ? 1024 / threads : 16; }
+
+template <typename TX, typename TR, typename TW, int NT, int VPT>
+__global__ void __launch_bounds__(NT, ring_ctas(NT, VPT)) block_norm_ring(NormParams p, int rows, int stages) {
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ __align__(8) uint64_t full[MAX_STAGES];
+    __shared__ __align__(16) float scratch[2][4][32];
+    constexpr int VEC = 8;
+    const int d = p.op.d, tid = threadIdx.x;
+    const uint32_t bx = d * sizeof(TX), br = d * sizeof(TR);
+    const bool gate_rows = p.gate_kind == ESP_GATE_ELEMENT;
+    const uint32_t stage_bytes = bx * (1 + (p.x2 != nullptr) + gate_rows) + (p.residual ? br : 0);
+    if (tid == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    pdl_launch_dependents();
+    pdl_wait();
+    const auto request = [&](int row, int s) {          // thread 0
+        uint32_t to = smem_addr(ring) + s * stage_bytes;
+        mbar_arrive_expect_tx(&full[s], stage_bytes);
+        bulk_g2s(to, static_cast<const TX*>(p.x) + row * p.x_stride, bx, &full[s]);
+        to += bx;
+        if (p.x2) bulk_g2s(to, static_cast<const TX*>(p.x2) + row * p.x2_stride, bx, &full[s]), to += bx;
+        if (gate_rows) bulk_g2s(to, static_cast<const TX*>(p.gate) + row * p.gate_stride, bx, &full[s]), to += bx;
+        if (p.residual) bulk_g2s(to, static_cast<const TR*>(p.residual) + row * p.residual_stride, br, &full[s]);
+    };
+    const int step = gridDim.x;
+    if (tid == 0)
+        for (int s = 0; s < stages && blockIdx.x + s * step < rows; ++s) request(blockIdx.x + s * step, s);
+    RowWeights<TW, VEC, VPT> w;
+    fetch_weights<TW, VEC, NT, VPT>(w, p);
+    int s = 0, phase = 0, parity = 0;
+    for (int row = blockIdx.x; row < rows; row += step) {
+        // A wait that gave up ends the CTA, all threads together, after a bounded wait for the copies still on their way.
+        if (!__syncthreads_and(mbar_wait(&full[s], phase))) {
+            if (tid == 0)
+                for (int k = 0; k < stages; ++k) mbar_wait(&full[k], k < s ? phase ^ 1 : phase);
+            return;
+        }
+        // that barrier also ends the row before: its stage can be filled again
+        if (tid == 0 && row != blockIdx.x) {
+            const int last = (s ? s : stages) - 1, next = row + (stages - 1) * step;
+            if (next < rows) request(next, last);
+        }
+        InStage<TX, TR, VEC> in;
+        in.x_ = ring + s * stage_bytes;
+        in.x2_ = in.x_ + bx;
+        in.gate_ = gate_rows ? in.x2_ + (p.x2 ? bx : 0) : static_cast<const unsigned char*>(p.gate);
+        in.res_ = in.x_ + stage_bytes - br;
+        norm_row<TX, TR, TW, VEC, NT, VPT, true>(p, row, in, w, scratch[parity]);
+        parity ^= 1;
+        if (++s == stages) s = 0, phase ^= 1;
+    }
+}
+
 constexpr int MAX_D = 49152;   // the row as fp32 in shared memory: 192 KB
 bool known_dtype(int t) { return t == F16 || t == BF16 || t == F32; }
 
@@ -295,12 +434,15 @@ bool vector_rows(const void* p, int dtype, long long stride) {
 
 struct RowsKernel {
     void (*run)(NormParams) = nullptr;
-    int threads = 0;
+    void (*ring)(NormParams, int, int) = nullptr;
+    int threads = 0, ctas = 0;      // of a CTA; CTAs of the ring's kernel an SM
 };
 
 template <typename TX, typename TR, typename TW, int VEC, int NT, int VPT>
 RowsKernel rows_instance() {
-    return {block_norm_rows<TX, TR, TW, VEC, NT, VPT>, NT};
+    if constexpr (VEC == 8)
+        return {block_norm_rows<TX, TR, TW, VEC, NT, VPT>, block_norm_ring<TX, TR, TW, NT, VPT>, NT, ring_ctas(NT, VPT)};
+    else return {block_norm_rows<TX, TR, TW, VEC, NT, VPT>, nullptr, NT, 0};
 }
 
 // The registers' kernel for this width, none where the row does not fit: the threads a row needs for one group each
@@ -309,6 +451,7 @@ RowsKernel rows_instance() {
 template <typename TX, typename TR, typename TW>
 RowsKernel rows_kernel(int d, bool vec) {
     if (vec) {
+        if (d <= 256) return rows_instance<TX, TR, TW, 8, 32, 1>();
         if (d <= 1024) return rows_instance<TX, TR, TW, 8, 128, 1>();
         if (d <= 2048) return rows_instance<TX, TR, TW, 8, 256, 1>();
         if (d <= 4096) return rows_instance<TX, TR, TW, 8, 512, 1>();
@@ -350,8 +493,16 @@ RowsKernel rows_kernel(const NormParams& p) {
     return rows_kernel<float>(p, vec);
 }
 
+// Bytes of one row's inputs (a stage of the ring).
+int row_bytes(const NormParams& p) {
+    const int x = p.x_dtype == F32 ? 4 : 2, r = p.r_dtype == F32 ? 4 : 2;
+    return p.op.d * (x * (1 + (p.x2 != nullptr) + (p.gate_kind == ESP_GATE_ELEMENT)) + (p.residual ? r : 0));
+}
+
 }  // namespace
 }  // namespace esp
+
+ESP_DEFINE_STATUS_READER(norms)
 
 extern "C" int esp_block_norm(const esp_block_norm_op_t* op, const void* x, long long x_stride, const void* x2,
                               long long x2_stride, int x_dtype, const void* residual, long long residual_stride,
@@ -381,6 +532,15 @@ extern "C" int esp_block_norm(const esp_block_norm_op_t* op, const void* x, long
     NormParams p{*op, x, x2, residual, gate, r_out, h_out, x_stride, x2_stride, residual_stride, gate_stride,
                  r_out_stride, h_out_stride, x_dtype, r_dtype, gate_kind, gate_dtype};
     if (const RowsKernel k = rows_kernel(p); k.run) {
+        const int stages = k.ring ? std::min(MAX_STAGES, (RING_BYTES / k.ctas - RING_FIXED) / row_bytes(p)) : 0;
+        if (rows > static_cast<long long>(k.ctas) * device_sms() && stages >= 2) {
+            const int smem = stages * row_bytes(p);
+            if (const int rc = allow_smem(k.ring, std::max(smem, 49153))) return rc;
+            if (const int rc = launch(k.ring, dim3(k.ctas * device_sms()), dim3(k.threads), smem, stream, true, p,
+                                      static_cast<int>(rows), stages))
+                return rc;
+            return ok();
+        }
         if (const int rc = launch(k.run, dim3(static_cast<unsigned>(rows)), dim3(k.threads), 0, stream, true, p)) return rc;
         return ok();
     }

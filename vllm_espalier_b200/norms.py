@@ -61,9 +61,9 @@ class BlockNorm:
                                        at.get("pre_w"), at.get("pre_b"))
         self._ref = C.addressof(self._op)
 
-    def _rows(self, t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
-        if t.shape != like.shape or t.device != like.device or t.dtype not in DTYPE:
-            raise ValueError(f"{name} must be fp16/bf16/fp32 {tuple(like.shape)} on {like.device}, got {t.dtype} "
+    def _rows(self, t: torch.Tensor, name: str, x: torch.Tensor) -> torch.Tensor:
+        if t.shape != x.shape or t.device != x.device or t.dtype not in DTYPE:
+            raise ValueError(f"{name} must be fp16/bf16/fp32 {tuple(x.shape)} on {x.device}, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
         return t if t.stride(1) == 1 else t.contiguous()
 
@@ -73,55 +73,62 @@ class BlockNorm:
         """x, x2 [rows, d] of one dtype, residual [rows, d]; gate [d], [rows, 1] or [rows, d]. Returns (r, h): r in the
         residual's dtype (x's without one), h in x's, None without the pre norm. out / normed: tensors to write r / h
         to (out may be the residual or x, normed may be x)."""
-        if x.dim() != 2 or x.shape[1] != self.d or not x.is_cuda or x.dtype not in DTYPE:
-            raise ValueError(f"x must be a CUDA fp16/bf16/fp32 [rows, {self.d}] tensor, got {x.dtype} "
-                             f"{tuple(x.shape)}")
-        rows, r_dtype = x.shape[0], x.dtype
-        if x.stride(1) != 1:
+        d, x_dtype = self.d, x.dtype
+        x_code = DTYPE.get(x_dtype)
+        if x.dim() != 2 or x.shape[1] != d or not x.is_cuda or x_code is None:
+            raise ValueError(f"x must be a CUDA fp16/bf16/fp32 [rows, {d}] tensor, got {x_dtype} {tuple(x.shape)}")
+        x_stride, step = x.stride()
+        if step != 1:
             x = x.contiguous()
+            x_stride = d
+        rows = x.shape[0]
         x2_ptr = x2_stride = residual_ptr = residual_stride = gate_ptr = gate_stride = kind = gate_dtype = 0
         if x2 is not None:
             x2 = self._rows(x2, "x2", x)
-            if x2.dtype != x.dtype:
-                raise ValueError(f"x2 must have x's dtype {x.dtype}, got {x2.dtype}")
+            if x2.dtype != x_dtype:
+                raise ValueError(f"x2 must have x's dtype {x_dtype}, got {x2.dtype}")
             x2_ptr, x2_stride = x2.data_ptr(), x2.stride(0)
+        r_like, r_dtype, r_code = x, x_dtype, x_code
         if residual is not None:
-            residual = self._rows(residual, "residual", x)
-            r_dtype, residual_ptr, residual_stride = residual.dtype, residual.data_ptr(), residual.stride(0)
+            r_like = residual = self._rows(residual, "residual", x)
+            residual_ptr, residual_stride, r_dtype = residual.data_ptr(), residual.stride(0), residual.dtype
+            r_code = DTYPE[r_dtype]
         if gate is not None:
             if gate.device != x.device or gate.dtype not in DTYPE:
                 raise ValueError(f"gate must be fp16/bf16/fp32 on {x.device}, got {gate.dtype} on {gate.device}")
-            if gate.shape == (self.d,):
+            if gate.shape == (d,):
                 kind, gate = GATE_CHANNEL, gate.contiguous()
             elif gate.shape == (rows, 1):
                 kind, gate_stride = GATE_ROW, gate.stride(0)
-            elif gate.shape == (rows, self.d):
+            elif gate.shape == (rows, d):
                 gate = gate if gate.stride(1) == 1 else gate.contiguous()
                 kind, gate_stride = GATE_ELEMENT, gate.stride(0)
             else:
-                raise ValueError(f"gate must be [{self.d}], [{rows}, 1] or [{rows}, {self.d}], got "
-                                 f"{tuple(gate.shape)}")
+                raise ValueError(f"gate must be [{d}], [{rows}, 1] or [{rows}, {d}], got {tuple(gate.shape)}")
             gate_ptr, gate_dtype = gate.data_ptr(), DTYPE[gate.dtype]
-        r = self._output(out, "out", x, r_dtype)
-        h, h_ptr, h_stride = None, 0, 0
+        if out is None:
+            out, r_stride = torch.empty_like(r_like, memory_format=torch.contiguous_format), d
+        else:
+            r_stride = self._given(out, "out", x, r_dtype)
+        h_ptr = h_stride = 0
         if self.has_pre:
-            h = self._output(normed, "normed", x, x.dtype)
-            h_ptr, h_stride = h.data_ptr(), h.stride(0)
+            if normed is None:
+                normed, h_stride = torch.empty_like(x, memory_format=torch.contiguous_format), d
+            else:
+                h_stride = self._given(normed, "normed", x, x_dtype)
+            h_ptr = normed.data_ptr()
         elif normed is not None:
             raise ValueError("normed given, but this BlockNorm has no pre norm")
         if rows:
-            check(lib().esp_block_norm(self._ref, x.data_ptr(), x.stride(0), x2_ptr, x2_stride, DTYPE[x.dtype],
-                                       residual_ptr, residual_stride, DTYPE[r_dtype], gate_ptr, kind, gate_dtype,
-                                       gate_stride, r.data_ptr(), r.stride(0), h_ptr, h_stride, rows,
-                                       stream_ptr(x.device)))
-        return r, h
+            check(lib().esp_block_norm(self._ref, x.data_ptr(), x_stride, x2_ptr, x2_stride, x_code, residual_ptr,
+                                       residual_stride, r_code, gate_ptr, kind, gate_dtype, gate_stride,
+                                       out.data_ptr(), r_stride, h_ptr, h_stride, rows, stream_ptr(x.device)))
+        return out, normed
 
     @staticmethod
-    def _output(t: torch.Tensor | None, name: str, x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-        if t is None:
-            return torch.empty(x.shape, dtype=dtype, device=x.device)
+    def _given(t: torch.Tensor, name: str, x: torch.Tensor, dtype: torch.dtype) -> int:
         if t.shape != x.shape or t.dtype != dtype or t.device != x.device or t.stride(1) != 1:
             raise ValueError(f"{name} must be {dtype} {tuple(x.shape)} on {x.device} with unit column stride")
-        return t
+        return t.stride(0)
 
     __call__ = forward
