@@ -16,6 +16,7 @@ int status_route(int reset);
 int status_moe(int reset);
 int status_ep(int reset);
 int status_norms(int reset);
+int status_verify(int reset);
 
 namespace {
 thread_local char t_msg[512] = "";
@@ -67,7 +68,8 @@ int esp_sm_count(void) { return esp::device_sms(); }
 int esp_device_status(int* status, int reset) {
     if (!status) return esp::set_error(ESP_ERR_INVALID, "esp_device_status: status is NULL");
     int v = 0;
-    for (int (*rd)(int) : {esp::status_dense, esp::status_route, esp::status_moe, esp::status_ep, esp::status_norms}) {
+    for (int (*rd)(int) : {esp::status_dense, esp::status_route, esp::status_moe, esp::status_ep, esp::status_norms,
+                          esp::status_verify}) {
         const int s = rd(reset);
         if (s < 0) return esp::set_error(ESP_ERR_CUDA, "esp_device_status: %s", cudaGetErrorString(cudaGetLastError()));
         if (!v) v = s;

@@ -194,6 +194,18 @@ __device__ __forceinline__ float4 ld_cluster_f4(const void* local, uint32_t rank
     return v;
 }
 
+// Four words into another CTA's shared memory, their 16 bytes counted on an mbarrier there (both given by this CTA's own
+// addresses of the same objects): who waits for the barrier's bytes sees the words, with no barrier of the cluster.
+__device__ __forceinline__ void st_async_v4(void* local, uint64_t* bar, uint32_t rank, uint32_t a, uint32_t b, uint32_t c,
+                                            uint32_t d) {
+    uint32_t to, on;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_addr(local)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(on) : "r"(smem_addr(bar)), "r"(rank));
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.u32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
+                 "r"(a), "r"(b), "r"(c), "r"(d), "r"(on)
+                 : "memory");
+}
+
 // Release/acquire fence at GPU scope. One thread executes it after a CTA barrier: the fence is cumulative over the
 // writes the barrier ordered before it, so the whole CTA's stores are published without a fence in every thread.
 __device__ __forceinline__ void fence_acq_rel_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }

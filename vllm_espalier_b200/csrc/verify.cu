@@ -33,8 +33,15 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int THREADS = 256, WARPS = THREADS / 32, PACKS = 4, OCTETS = 2, SINGLES = 8, RESIDENT = 4;
+constexpr int MAX_SEGMENTS = 16, SEGMENT = 16384, FILL = 1000;
 constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // exp((l - m) / T) as 2^((l - m) c), c = log2(e) / T: 1 at the row's largest logit m, also where that is +inf (the row's
 // mass is then shared by its infinite logits), 0 for -inf and NaN.
@@ -61,33 +68,136 @@ __device__ __forceinline__ Part joined(Part a, Part b, float c) {
     return {m, z, a.m == b.m ? min(a.at, b.at) : a.m > b.m ? a.at : b.at, 0};
 }
 
-// The join of the CTA's threads, in thread 0 (a barrier inside).
-__device__ __forceinline__ Part block_part(Part t, float c, bool places, Part* warps) {
-    float m = t.m;
+// What a CTA shares: its warps' values of a round, the cluster's of two rounds in turn, and what came of a round.
+struct Shared {
+    Part warps[MAX_SEGMENTS * WARPS];       // [own segment][warp]
+    Part table[2][MAX_SEGMENTS];
+    Part result;
+    int gave_up;                            // a wait of the exchange did
+    uint64_t full[2];                       // of the tables, armed for their next round
+};
+
+// What the CTAs of a cluster tell one another. In a round each warp puts a value into its CTA's `warps`; the CTA's first
+// warp joins them, stores one value for each of the CTA's segments into every CTA's table (its place by segment, so what
+// is made of the table does not depend on how many CTAs share the segments), counted there on the round's mbarrier, waits
+// for its own table and joins that. Two tables in turn: a CTA gives to round r + 2 only after it has the whole of round
+// r + 1, which every CTA gave to after it had read round r.
+struct Exchange {
+    Shared& sh;
+    int ctas, segments, own;        // own: segments of this CTA
+    int from;                       // the first of them
+    int round = 0;
+
+    __device__ __forceinline__ void arm(int r) {
+        mbar_arrive_expect_tx(&sh.full[r], segments * static_cast<uint32_t>(sizeof(Part)));
+    }
+
+    // The first warp, all lanes: the round's table once it is whole (NULL after a wait that gave up).
+    __device__ __forceinline__ const Part* whole(int r) {
+        const bool there = mbar_wait(&sh.full[r & 1], (r >> 1) & 1);
+        if (threadIdx.x == 0) arm(r & 1);
+        if (__all_sync(0xffffffffu, there)) return sh.table[r & 1];
+        if (threadIdx.x == 0) sh.gave_up = 1;
+        return nullptr;
+    }
+    __device__ __forceinline__ void give(int r, int segment, int to, uint32_t a, uint32_t b, uint32_t c) {
+        st_async_v4(&sh.table[r & 1][segment], &sh.full[r & 1], to, a, b, c, 0);
+    }
+
+    // The join of the parts that the cluster's warps put into `warps`, in every thread. After a wait that gave up: an
+    // empty part.
+    __device__ __forceinline__ Part part(float c) {
+        const int lane = threadIdx.x & 31, r = round++;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            for (int i = 0; i < own; i += 32 / WARPS) {     // four segments at once, eight lanes each
+                const int s = i + lane / WARPS;
+                Part t = {-INFINITY, 0.0f, INT_MAX, 0};
+                if (s < own) t = sh.warps[i * WARPS + lane];
+                t = lanes_part(t, c, WARPS / 2);
+                if (s < own)
+                    for (int to = lane % WARPS; to < ctas; to += WARPS)
+                        give(r, from + s, to, __float_as_uint(t.m), __float_as_uint(t.z), t.at);
+            }
+            const Part* table = whole(r);
+            Part t = {-INFINITY, 0.0f, INT_MAX, 0};
+            if (table && lane < segments) t = table[lane];
+            t = lanes_part(t, c, MAX_SEGMENTS / 2);
+            if (lane == 0) sh.result = t;
+        }
+        __syncthreads();
+        return sh.result;
+    }
+
+    // The largest of the keys that this CTA's and the others' warps put into `warps` (of the first own segment).
+    __device__ __forceinline__ unsigned long long largest() {
+        const int lane = threadIdx.x & 31, r = round++;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            unsigned long long key = lane < WARPS ? as_key(sh.warps[lane]) : 0;
+            key = lanes_max(key, 16);       // in every lane: each sends it to a CTA of its own
+            if (lane < ctas)
+                for (int s = 0; s < own; ++s)
+                    give(r, from + s, lane, static_cast<uint32_t>(key >> 32), static_cast<uint32_t>(key), 0);
+            const Part* table = whole(r);
+            key = lanes_max(table && lane < segments ? as_key(table[lane]) : 0, MAX_SEGMENTS / 2);
+            if (lane == 0) sh.result = {__uint_as_float(static_cast<uint32_t>(key >> 32)),
+                                        __uint_as_float(static_cast<uint32_t>(key)), 0, 0};
+        }
+        __syncthreads();
+        return as_key(sh.result);
+    }
+
+    static __device__ __forceinline__ unsigned long long as_key(const Part& t) {
+        return static_cast<unsigned long long>(__float_as_uint(t.m)) << 32 | __float_as_uint(t.z);
+    }
+    // Over groups of 2 * half lanes from lane 0 on.
+    static __device__ __forceinline__ Part lanes_part(Part t, float c, int half) {
 #pragma unroll
-    for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-    float z = t.m == m ? t.z : t.z * ex2((t.m - m) * c);
-#pragma unroll
-    for (int k = 16; k; k >>= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
-    int at = 0;
-    if (places) at = __reduce_min_sync(0xffffffffu, t.m == m ? t.at : INT_MAX);
-    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = {m, z, at, 0};
-    __syncthreads();
-    t = {-INFINITY, 0.0f, INT_MAX, 0};
-    if (threadIdx.x < 32) {
-        if (threadIdx.x < WARPS) t = warps[threadIdx.x];
-#pragma unroll
-        for (int k = WARPS / 2; k; k >>= 1)
+        for (int k = half; k; k >>= 1)
             t = joined(t, {__shfl_xor_sync(0xffffffffu, t.m, k), __shfl_xor_sync(0xffffffffu, t.z, k),
                            __shfl_xor_sync(0xffffffffu, t.at, k), 0}, c);
+        return t;
     }
-    return t;
-}
+    static __device__ __forceinline__ unsigned long long lanes_max(unsigned long long key, int half) {
+#pragma unroll
+        for (int k = half; k; k >>= 1) {
+            const unsigned long long o = __shfl_xor_sync(0xffffffffu, key, k);
+            key = o > key ? o : key;
+        }
+        return key;
+    }
+};
 
 template <typename T>
 struct alignas(16) Pack {
     T e[16 / sizeof(T)];
 };
+
+template <typename T>
+struct alignas(16) Octet {
+    T e[8];
+};
+
+// The largest of a thread's logits, NaN aside, two at an instruction where they are 16-bit.
+__device__ __forceinline__ float largest_of(const Pack<float> (&k)[PACKS]) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < PACKS; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, k[u].e[e]);
+    return top;
+}
+template <typename T>
+__device__ __forceinline__ float largest_of(const Pack<T> (&k)[PACKS]) {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 top = *reinterpret_cast<const T2*>(&k[0].e[0]);
+#pragma unroll
+    for (int u = 0; u < PACKS; ++u)
+#pragma unroll
+        for (int e = u ? 0 : 2; e < 8; e += 2) top = __hmax2(top, *reinterpret_cast<const T2*>(&k[u].e[e]));
+    return fmaxf(f32(top.x), f32(top.y));
+}
 
 // This thread's share of the part [lo, hi) of a row, in one pass. The thread keeps the largest logit m that it has met
 // and the sum of 2^(l c - mc) with mc = m c rounded; a larger m rescales the sum by 2^(mc - mc'). The rounding of mc is
@@ -96,88 +206,122 @@ struct alignas(16) Pack {
 // FLOOR comes out with a sum that is NaN, infinite or 0, which the caller sees and takes careful_part instead.
 constexpr float FLOOR = -1e30f;
 template <typename T>
-__device__ __forceinline__ Part fast_part(const T* row, int lo, int hi, float c, bool places) {
-    constexpr int N = 16 / sizeof(T), UNROLL = 4;
+__device__ __forceinline__ Part fast_part(const T* row, int lo, int hi, float c) {
+    constexpr int N = 16 / sizeof(T);
     float m = FLOOR, mc = 0.0f, z = 0.0f;
-    int first = -1;         // where the pack starts among whose logits the largest was first met
-    const auto take = [&](const Pack<T>& k, int v) {
-        float l[N], top = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < N; ++e) top = fmaxf(top, l[e] = f32(k.e[e]));
-        if (top > m) {
-            const float next = top * c;
-            z = first < 0 ? 0.0f : z * ex2(mc - next);
-            m = top, mc = next, first = v;
-        }
-#pragma unroll
-        for (int e = 0; e < N; ++e) z += ex2(fmaf(l[e], c, -mc));
+    int first = -1;         // where the batch starts among whose logits the largest was first met
+    const auto raise = [&](float top, int v) {
+        const float next = top * c;
+        z = first < 0 ? 0.0f : z * ex2(mc - next);
+        m = top, mc = next, first = v;
     };
     // 16-byte loads from the first boundary on, the ends one by one
     const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row + lo) % 16 / sizeof(T));
     const int head = min(hi, lo + (off ? N - off : 0)), packs = (hi - head) / N, tail = head + packs * N;
     const auto single = [&](int v) {
         const float l = f32(row[v]);
-        if (l > m) {
-            const float next = l * c;
-            z = first < 0 ? 0.0f : z * ex2(mc - next);
-            m = l, mc = next, first = v;
-        }
+        if (l > m) raise(l, v);
         z += ex2(fmaf(l, c, -mc));
+    };
+    // PACKS packs, THREADS apart, from pack i on; those past the end read as the batch's first once more and weigh nothing
+    const auto batch = [&](int i, auto whole) {
+        Pack<T> k[PACKS];
+#pragma unroll
+        for (int u = 0; u < PACKS; ++u) {
+            const bool in = whole || u == 0 || i + u * THREADS < packs;
+            k[u] = *reinterpret_cast<const Pack<T>*>(row + head + (in ? i + u * THREADS : i) * N);
+        }
+        const float top = largest_of(k);
+        if (top > m) raise(top, head + i * N);
+#pragma unroll
+        for (int u = 0; u < PACKS; ++u)
+            if (whole || u == 0 || i + u * THREADS < packs)
+#pragma unroll
+                for (int e = 0; e < N; ++e) z += ex2(fmaf(f32(k[u].e[e]), c, -mc));
     };
     // before the packs, so that a thread meets its places in order
     if (lo + static_cast<int>(threadIdx.x) < head) single(lo + threadIdx.x);
     int i = threadIdx.x;
-    for (; i + (UNROLL - 1) * THREADS < packs; i += UNROLL * THREADS) {
-        Pack<T> k[UNROLL];
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) k[u] = *reinterpret_cast<const Pack<T>*>(row + head + (i + u * THREADS) * N);
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) take(k[u], head + (i + u * THREADS) * N);
-    }
-    for (; i < packs; i += THREADS) take(*reinterpret_cast<const Pack<T>*>(row + head + i * N), head + i * N);
+    for (; i + (PACKS - 1) * THREADS < packs; i += PACKS * THREADS) batch(i, std::true_type());
+    if (i < packs) batch(i, std::false_type());
     if (tail + static_cast<int>(threadIdx.x) < hi) single(tail + threadIdx.x);
     if (first >= 0) z *= ex2(-fmaf(m, c, -mc));
-    int at = first;
-    if (places && first >= 0)
-        while (f32(row[at]) != m) ++at;     // met: a logit of the pack at `first` equals m
-    return {m, z, first < 0 ? INT_MAX : at, 0};
+    return {m, z, first < 0 ? INT_MAX : first, 0};
 }
 
-// The same for any row: NaN counts as -inf, weights as weight() has them. The whole CTA's part, in every thread.
+// The lowest place of m among the logits of the batch that starts at v (a single one's place: that place), for a thread
+// that met m there.
 template <typename T>
-__device__ __noinline__ Part careful_part(const T* row, int lo, int hi, float c, Part* warps) {
-    Part t = {-INFINITY, 0.0f, INT_MAX, 0};
-    for (int v = lo + threadIdx.x; v < hi; v += THREADS) {
-        const float l = f32(row[v]);
-        if (l > t.m) t = {l, 0.0f, v, 0};
-    }
-    __shared__ Part all;
-    t = block_part(t, c, true, warps);      // no sums yet: only the largest and its place
-    if (threadIdx.x == 0) all = t;
-    __syncthreads();
-    t = all;
-    float z = 0.0f;
-    if (t.m > -INFINITY)
-        for (int v = lo + threadIdx.x; v < hi; v += THREADS) z += weight(f32(row[v]), t.m, c);
-    const Part sum = block_part({0.0f, z, 0, 0}, c, false, warps);
-    if (threadIdx.x == 0) all.z = sum.z;
-    __syncthreads();
-    t = all;
-    __syncthreads();
-    return t;
+__device__ __forceinline__ int place_of(const T* row, int v, int hi, float m) {
+    constexpr int N = 16 / sizeof(T);
+    for (int u = 0; u < PACKS; ++u)
+        for (int e = 0; e < N; ++e) {
+            const int at = v + u * THREADS * N + e;
+            if (at < hi && f32(row[at]) == m) return at;
+        }
+    return v;
 }
 
-// Every CTA of the cluster gives its part (of thread 0) and gets the row's, joined in the order of the ranks: one cluster
-// barrier. `slot` is written again only after another barrier of the cluster.
-__device__ __forceinline__ Part cluster_part(Part mine, float c, Part* slot, int ctas) {
-    if (threadIdx.x == 0) *slot = mine;
-    cluster_sync_all();
-    Part t = {-INFINITY, 0.0f, INT_MAX, 0};
-    for (int r = 0; r < ctas; ++r) {
-        const float4 q = ld_cluster_f4(slot, r);
-        t = joined(t, {q.x, q.y, __float_as_int(q.z), 0}, c);
+// The largest of a warp's values (no NaN), in every lane, by an integer whose order is the value's.
+__device__ __forceinline__ float warp_max(float v) {
+    const unsigned u = __float_as_uint(v);
+    const unsigned r = __reduce_max_sync(0xffffffffu, u & 0x80000000u ? ~u : u | 0x80000000u);
+    return __uint_as_float(r & 0x80000000u ? r & 0x7fffffffu : ~r);
+}
+
+// The join of a warp's threads into the CTA's table, for its i-th segment. `place`: a thread's lowest place of its
+// largest, asked of the threads that have the warp's largest only.
+template <typename Place>
+__device__ __forceinline__ void put(Shared& sh, int i, Part t, float c, bool places, Place place) {
+    const float m = warp_max(t.m);
+    float z = t.m == m ? t.z : t.z * ex2((t.m - m) * c);
+#pragma unroll
+    for (int k = 16; k; k >>= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
+    int at = INT_MAX;
+    if (places) at = __reduce_min_sync(0xffffffffu, t.m == m && t.at != INT_MAX ? place(t) : INT_MAX);
+    if ((threadIdx.x & 31) == 0) sh.warps[i * WARPS + (threadIdx.x >> 5)] = {m, z, at, 0};
+}
+
+// The vocabulary in segments of `size` ids; this CTA's are [from, from + count).
+struct Segments {
+    int from, count, size, vocab;
+    __device__ __forceinline__ int lo(int i) const { return min(vocab, (from + i) * size); }
+    __device__ __forceinline__ int hi(int i) const { return min(vocab, (from + i + 1) * size); }
+};
+
+// The row's part for any row: NaN counts as -inf, weights as weight() has them. Takes CAREFUL_ROUNDS of the exchange,
+// which the caller adds to its own count.
+constexpr int CAREFUL_ROUNDS = 2;
+template <typename T>
+__device__ __noinline__ Part careful_part(const T* row, Segments own, float c, Exchange exchange) {
+    const auto as_met = [](const Part& t) { return t.at; };
+    for (int i = 0; i < own.count; ++i) {
+        Part t = {-INFINITY, 0.0f, INT_MAX, 0};
+        for (int v = own.lo(i) + threadIdx.x; v < own.hi(i); v += THREADS) {
+            const float l = f32(row[v]);
+            if (l > t.m) t = {l, 0.0f, v, 0};
+        }
+        put(exchange.sh, i, t, c, true, as_met);
     }
-    return t;
+    Part all = exchange.part(c);
+    for (int i = 0; i < own.count; ++i) {
+        Part t = {0.0f, 0.0f, INT_MAX, 0};
+        if (all.m > -INFINITY)
+            for (int v = own.lo(i) + threadIdx.x; v < own.hi(i); v += THREADS) t.z += weight(f32(row[v]), all.m, c);
+        put(exchange.sh, i, t, c, false, as_met);
+    }
+    all.z = exchange.part(c).z;
+    return all;
+}
+
+// Asks for the whole 16-byte blocks of a range into L2 (a hint: at most 64 KB an instruction's worth at a time).
+__device__ __forceinline__ void prefetch_l2(const void* p, size_t bytes) {
+    uintptr_t a = (reinterpret_cast<uintptr_t>(p) + 15) / 16 * 16;
+    const uintptr_t end = (reinterpret_cast<uintptr_t>(p) + bytes) / 16 * 16;
+    for (; a < end; a += 65536) {
+        const uint32_t n = static_cast<uint32_t>(end - a < 65536 ? end - a : 65536);
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a), "r"(n) : "memory");
+    }
 }
 
 struct NoProbs {};      // the drafter chose its token outright
@@ -187,25 +331,162 @@ __device__ __forceinline__ float draft_prob(const Q* q, long long i) {
     else return f32(q[i]);
 }
 
-// A cluster of `ctas` CTAs a request, each with its part of the vocabulary: rows in order until a drafted token falls.
-// Every CTA reads the same parts and so takes the same decisions.
+// A row's weights in the race: p(v) = e(l) scale with e(l) = 2^(l c - mc), mc = m c rounded and its rounding in `scale`;
+// SAFE: weight() instead, for rows that careful_part summed.
+struct Weights {
+    float m, c, mc, scale;
+    template <bool SAFE>
+    __device__ __forceinline__ float e(float l) const {
+        return SAFE ? weight(l, m, c) : ex2(fmaf(l, c, -mc));
+    }
+};
+
+// A thread's best of the race so far: the largest max(p - q, 0) / noise and where it was met.
+struct Best {
+    float top = 0.0f;
+    int at = -1;
+};
+
+// The race over [lo, hi) from w: many loads are asked for before the first is used, a thread compares eight scores at
+// once and `at` is where its eight consecutive ids start (or a single id). SUBTRACT: a drafted token was turned down and
+// the drafter's probabilities are taken off.
+template <bool SAFE, bool SUBTRACT, typename T, typename Q>
+__device__ __forceinline__ void race(Best& best, const T* row, const Q* q, const float* noise, int out, int lo, int hi,
+                                     const Weights& wt) {
+    using O = std::conditional_t<SUBTRACT, Q, float>;
+    const auto score = [&](T l, float e, float qv) { return fmaf(wt.e<SAFE>(f32(l)), wt.scale, SUBTRACT ? -qv : 0.0f) * rcp(e); };
+    int v = lo;
+    if ((reinterpret_cast<uintptr_t>(row + lo) | reinterpret_cast<uintptr_t>(noise + lo) |
+         (SUBTRACT ? reinterpret_cast<uintptr_t>(q) + lo * sizeof(O) : 0)) % 16 == 0) {
+        const int groups = (hi - lo) / 8;
+        const auto batch = [&](int g, auto whole) {
+            Octet<T> l[OCTETS];
+            Octet<float> e[OCTETS];
+            [[maybe_unused]] Octet<O> o[OCTETS];
+#pragma unroll
+            for (int u = 0; u < OCTETS; ++u) {
+                const int at = lo + (whole || g + u * THREADS < groups ? g + u * THREADS : g) * 8;
+                l[u] = *reinterpret_cast<const Octet<T>*>(row + at);
+                e[u] = *reinterpret_cast<const Octet<float>*>(noise + at);
+                if constexpr (SUBTRACT) o[u] = *reinterpret_cast<const Octet<O>*>(q + at);
+            }
+#pragma unroll
+            for (int u = 0; u < OCTETS; ++u) {
+                const int at = lo + (whole || g + u * THREADS < groups ? g + u * THREADS : g) * 8;
+                float s[8], top = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if constexpr (SUBTRACT) s[j] = score(l[u].e[j], e[u].e[j], f32(o[u].e[j]));
+                    else s[j] = score(l[u].e[j], e[u].e[j], 0.0f);
+                }
+                if (!SUBTRACT && static_cast<unsigned>(out - at) < 8u) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (at + j == out) s[j] = 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, s[j]);
+                if (top > best.top) best = {top, at};
+            }
+        };
+        int g = threadIdx.x;
+        for (; g + (OCTETS - 1) * THREADS < groups; g += OCTETS * THREADS) batch(g, std::true_type());
+        if (g < groups) batch(g, std::false_type());
+        v = lo + groups * 8;
+    }
+    for (v += threadIdx.x; v < hi; v += SINGLES * THREADS) {
+        T l[SINGLES];
+        float e[SINGLES];
+        O o[SINGLES];
+#pragma unroll
+        for (int u = 0; u < SINGLES; ++u) {
+            const int at = min(v + u * THREADS, hi - 1);        // past the end: an id that was met
+            l[u] = row[at];
+            e[u] = noise[at];
+            if constexpr (SUBTRACT) o[u] = q[at];
+        }
+#pragma unroll
+        for (int u = 0; u < SINGLES; ++u) {
+            const int at = min(v + u * THREADS, hi - 1);
+            float s;
+            if constexpr (SUBTRACT) s = score(l[u], e[u], f32(o[u]));
+            else s = at == out ? 0.0f : score(l[u], e[u], 0.0f);
+            if (s > best.top) best = {s, at};
+        }
+    }
+}
+
+// The warp's best of the race over the CTA's segments, as a key in the CTA's table: the largest score, the lowest id among
+// equals, 0 without a candidate. `out`: an id out of the race (-1: none).
+template <bool SAFE, bool SUBTRACT, typename T, typename Q>
+__device__ __forceinline__ void race_all(Shared& sh, const T* row, const Q* q, const float* noise, int out, const Segments& own,
+                                         const Weights& wt) {
+    Best best;
+    for (int i = 0; i < own.count; ++i)
+        race<SAFE, SUBTRACT>(best, row, q, noise, out, own.lo(i), own.hi(i), wt);
+    const float top = warp_max(best.top);
+    int id = INT_MAX;
+    if (best.at >= 0 && best.top == top) {      // which of the eight (or of the one and those after it) it was
+        id = best.at;
+        for (int j = 0; j < 8 && best.at + j < own.vocab; ++j) {
+            const int v = best.at + j;
+            float qv = 0.0f;
+            if constexpr (SUBTRACT) qv = f32(q[v]);
+            const float s = fmaf(wt.e<SAFE>(f32(row[v])), wt.scale, SUBTRACT ? -qv : 0.0f) * rcp(noise[v]);
+            if (v != out && s == top) {
+                id = v;
+                break;
+            }
+        }
+    }
+    id = __reduce_min_sync(0xffffffffu, id);
+    if ((threadIdx.x & 31) == 0) {
+        const unsigned long long key = id == INT_MAX ? 0 : score_key(top, id);
+        sh.warps[threadIdx.x >> 5] = {__uint_as_float(static_cast<uint32_t>(key >> 32)),
+                                      __uint_as_float(static_cast<uint32_t>(key)), 0, 0};
+    }
+}
+
+struct Split {      // a request's vocabulary over segments and CTAs
+    int ctas_log2, segments, own, size;
+    bool ahead;
+};
+
+// A cluster of CTAs a request, each with its share of the vocabulary's segments: rows in order until a drafted token falls.
+// Every CTA reads the same joined parts and so takes the same decisions.
 template <typename T, typename Q>
-__global__ void __launch_bounds__(THREADS, 2) verify_kernel(VerifyParams p, int ctas) {
-    __shared__ Part warps[WARPS], parts[5];      // parts: two rows' in turn, two careful ones', the last resort's
-    __shared__ alignas(16) unsigned long long best_key[2];
-    constexpr bool ONE_HOT = std::is_same_v<Q, NoProbs>;
+__global__ void __launch_bounds__(THREADS, RESIDENT) verify_kernel(VerifyParams p, Split split) {
+    __shared__ Shared sh;
+    constexpr bool GIVEN = !std::is_same_v<Q, NoProbs>;
+    const int b = blockIdx.x >> split.ctas_log2, ctas = 1 << split.ctas_log2, rank = blockIdx.x & (ctas - 1);
+    const int V = p.vocab, width = p.max_drafts + 1;
+    const Segments own{rank * split.own, split.own, split.size, V};
+    const int lo = own.lo(0), hi = own.hi(own.count - 1);
+    const float* noise = p.noise + b * p.noise_stride;
+    Exchange exchange{sh, ctas, split.segments, own.count, own.from};
+    if (threadIdx.x == 0) {
+        sh.gave_up = 0;
+        for (int r = 0; r < 2; ++r) {
+            mbar_init(&sh.full[r], 1);
+            fence_mbar_init();
+            exchange.arm(r);
+        }
+        prefetch_l2(noise + lo, static_cast<size_t>(hi - lo) * sizeof(float));
+    }
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.x / ctas, rank = blockIdx.x % ctas, V = p.vocab, width = p.max_drafts + 1;
-    const int share = (V + 8 * ctas - 1) / (8 * ctas) * 8, lo = min(V, rank * share), hi = min(V, lo + share);
-    const bool writes = rank == 0 && threadIdx.x == 0;
-    const long long at = p.starts[b], first = at + b;
-    const long long k_all = static_cast<long long>(p.starts[b + 1]) - at;
+    const long long at = p.starts[b], next = p.starts[b + 1];
+    const float t = p.temperature ? p.temperature[b] : 1.0f;
+    cluster_sync_all();     // every CTA of the cluster is there, its barriers armed, before the first store into it
+    const long long first = at + b, k_all = next - at;
     const bool fits = at >= 0 && k_all >= 0 && at + k_all <= p.n_drafts && first + k_all < p.rows;
     const int k = static_cast<int>(min(k_all, static_cast<long long>(p.max_drafts)));
-    const float t = p.temperature ? p.temperature[b] : 1.0f;
     const bool greedy = !(t > 0.0f);
     const float c = greedy ? LOG2E : LOG2E / fminf(fmaxf(t, 1e-30f), 1e30f);
+    const bool fast = c >= 1e-6f && c <= 1e6f;
+    if (split.ahead && fits && threadIdx.x <= min(k, 31))
+        prefetch_l2(static_cast<const T*>(p.logits) + (first + threadIdx.x) * p.stride + lo,
+                    static_cast<size_t>(hi - lo) * sizeof(T));
     int* tokens = p.tokens + static_cast<size_t>(b) * width;
     float* probs = p.probs + static_cast<size_t>(b) * width;
 
@@ -213,91 +494,78 @@ __global__ void __launch_bounds__(THREADS, 2) verify_kernel(VerifyParams p, int 
     float token_p = 0.0f;
     for (int i = 0; fits && i <= k; ++i) {
         const T* row = static_cast<const T*>(p.logits) + (first + i) * p.stride;
-        const Q* q = static_cast<const Q*>(p.draft_probs) + (ONE_HOT ? 0 : (at + i) * p.probs_stride);
-        int d = -1;
+        const Q* q = static_cast<const Q*>(p.draft_probs) + (GIVEN ? (at + i) * p.probs_stride : 0);
+        int d = i < k ? p.drafts[at + i] : -1;
+        if (fast)
+            for (int s = 0; s < own.count; ++s) {
+                const int end = own.hi(s);
+                put(sh, s, fast_part(row, own.lo(s), end, c), c, greedy,
+                    [&](const Part& t) { return place_of(row, t.at, end, t.m); });
+            }
+        // asked for here, the drafted token's values arrive while the parts are joined
         float ld = 0.0f, qd = 0.0f, u = 0.0f;
-        if (i < k) {
-            d = p.drafts[at + i];
-            if (d < 0 || d >= V) d = -1;
-            else ld = f32(row[d]), qd = draft_prob(q, d), u = p.uniform[at + i];
-        }
+        if (d < 0 || d >= V) d = -1;
+        else ld = f32(row[d]), qd = draft_prob(q, d), u = p.uniform[at + i];
         n = i;
         Part all = {-INFINITY, 0.0f, INT_MAX, 0};
-        if (c >= 1e-6f && c <= 1e6f)
-            all = cluster_part(block_part(fast_part(row, lo, hi, c, greedy), c, greedy, warps), c, &parts[i & 1], ctas);
+        if (fast) all = exchange.part(c);
+        bool safe = false;
         if (!(all.z > 0.0f && all.z < INFINITY)) {
-            all = cluster_part(careful_part(row, lo, hi, c, warps), c, &parts[2 + (i & 1)], ctas);
+            safe = true;
+            all = careful_part(row, own, c, exchange);
+            exchange.round += CAREFUL_ROUNDS;
             if (all.m == -INFINITY) break;      // nothing left to choose from
         }
         const float m = all.m, inv_z = 1.0f / all.z;
         const float pd = d >= 0 ? weight(ld, m, c) * inv_z : 0.0f;
         if (d >= 0 && (greedy ? d == all.at : u * qd < pd)) {
-            if (writes) tokens[i] = d, probs[i] = pd;
+            if (rank == 0 && threadIdx.x == 0) tokens[i] = d, probs[i] = pd;
             continue;
         }
-        if (greedy) {
-            token = all.at;
-            token_p = inv_z;
-            break;
-        }
-        // The race: the largest w / noise, the lowest id among equals.
-        const float* noise = p.noise + b * p.noise_stride;
-        const bool fell = i < k;
-        unsigned long long key = 0;
-        {
-            float top = -1.0f;
-            int id = 0;
-            for (int v = lo + threadIdx.x; v < hi; v += THREADS) {
-                float w = weight(f32(row[v]), m, c) * inv_z;
-                if (fell) {
-                    if (ONE_HOT) w = v == d ? 0.0f : w;
-                    else w -= draft_prob(q, v);
+        token = all.at;
+        if (!greedy) {
+            const float mc = m * c;
+            const Weights wt{m, c, mc, safe ? inv_z : inv_z * ex2(-fmaf(m, c, -mc))};
+            const int out = GIVEN ? -1 : d;
+            if (GIVEN && i < k) {
+                if constexpr (GIVEN) {
+                    if (safe) race_all<true, true>(sh, row, q, noise, out, own, wt);
+                    else race_all<false, true>(sh, row, q, noise, out, own, wt);
                 }
-                const float score = __fdividef(w, noise[v]);
-                if (w > 0.0f && score > top) top = score, id = v;
+            } else {
+                if (safe) race_all<true, false>(sh, row, q, noise, out, own, wt);
+                else race_all<false, false>(sh, row, q, noise, out, own, wt);
             }
-            if (top >= 0.0f) key = score_key(top, id);
-        }
-#pragma unroll
-        for (int j = 16; j; j >>= 1) {
-            const unsigned long long o = __shfl_xor_sync(0xffffffffu, key, j);
-            key = o > key ? o : key;
-        }
-        unsigned long long* keys = reinterpret_cast<unsigned long long*>(warps);
-        if ((threadIdx.x & 31) == 0) keys[threadIdx.x >> 5] = key;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < WARPS; ++w) key = keys[w] > key ? keys[w] : key;
-            best_key[0] = key;
-        }
-        cluster_sync_all();
-        key = 0;
-        for (int r = 0; r < ctas; ++r) {
-            const float4 o = ld_cluster_f4(best_key, r);
-            const unsigned long long other =
-                static_cast<unsigned long long>(__float_as_uint(o.y)) << 32 | __float_as_uint(o.x);
-            key = other > key ? other : key;
-        }
-        if (key) {
+            const unsigned long long key = exchange.largest();
             token = key_id(key);
-        } else {        // no weight left: the target's likeliest token
-            all = cluster_part(careful_part(row, lo, hi, c, warps), c, &parts[4], ctas);
-            token = all.at;
+            if (!key) {         // no weight left: the target's likeliest token
+                token = careful_part(row, own, c, exchange).at;
+                if (token == INT_MAX) token = -1;       // (a wait of the exchange gave up)
+            }
         }
-        token_p = weight(f32(row[token]), m, c) * inv_z;
+        if (token >= 0) token_p = weight(f32(row[token]), m, c) * inv_z;
         break;
     }
-    if (writes) p.accepted[b] = n;
-    if (rank == 0)
+    if (rank == 0) {
+        if (threadIdx.x == 0) p.accepted[b] = n;
         for (int i = n + threadIdx.x; i < width; i += THREADS) {
             tokens[i] = i == n ? token : -1;
             probs[i] = i == n ? token_p : 0.0f;
         }
-    cluster_sync_all();     // no CTA leaves while another may read its shared memory
+    }
+    cluster_sync_all();     // no CTA leaves while another may store into its shared memory,
+    if (sh.gave_up) {       // nor, where it stopped waiting for a store, before that has had time to land
+        const uint64_t from = global_ns();
+        while (global_ns() - from < 20000) __nanosleep(1000);
+    }
 }
 
-// CTAs a request, by the vocabulary alone, so that a row's sums do not depend on the batch.
-int cluster_ctas(int vocab) { return vocab > 32768 ? 8 : vocab > 16384 ? 4 : vocab > 8192 ? 2 : 1; }
+// Segments of a vocabulary: by its size alone, so that a row's sums do not depend on the batch.
+int vocab_segments(int vocab) {
+    int n = 1;
+    while (n < MAX_SEGMENTS && vocab > n * SEGMENT) n *= 2;
+    return n;
+}
 
 template <typename T>
 auto kernel_of(bool given, int probs_dtype) {
@@ -310,6 +578,8 @@ bool known_dtype(int t) { return t == F16 || t == BF16 || t == F32; }
 
 }  // namespace
 }  // namespace esp
+
+ESP_DEFINE_STATUS_READER(verify)
 
 extern "C" int esp_verify(const void* logits, int dtype, long long stride, long long rows, int vocab, const int* starts,
                           int requests, const int* drafts, const float* uniform, long long n_drafts,
@@ -331,10 +601,17 @@ extern "C" int esp_verify(const void* logits, int dtype, long long stride, long 
     const auto kernel = dtype == F32    ? kernel_of<float>(draft_probs, probs_dtype)
                         : dtype == BF16 ? kernel_of<__nv_bfloat16>(draft_probs, probs_dtype)
                                         : kernel_of<__half>(draft_probs, probs_dtype);
-    const int ctas = cluster_ctas(vocab);
-    ESP_REQUIRE(requests <= INT_MAX / ctas, ESP_ERR_INVALID, "esp_verify: %d requests", requests);
-    if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(requests * ctas)), dim3(THREADS), 0, stream, true,
-                                      ctas, p, ctas))
+    const int segments = vocab_segments(vocab), sms = device_sms();
+    int log2 = 0;
+    while (1 << log2 < segments && (static_cast<long long>(requests) << log2) < FILL * sms) ++log2;
+    const int ctas = 1 << log2;
+    ESP_REQUIRE(requests <= INT_MAX >> log2, ESP_ERR_INVALID, "esp_verify: %d requests", requests);
+    if (ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return cuda_status("esp_verify: cluster of 16");
+    const Split split{log2, segments, segments >> log2, (vocab + 8 * segments - 1) / (8 * segments) * 8,
+                      requests * ctas <= sms};
+    if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(requests) << log2), dim3(THREADS), 0, stream, true,
+                                      ctas, p, split))
         return rc;
     return ok();
 }
