@@ -1,5 +1,21 @@
 // Low-rank adapters of many requests at once beside a shared projection.
+//
+// out[t] = y[t] + scale (x[t] A^T) B^T. Rows are grouped by adapter into tiles of M rows; a cluster of eight CTAs takes a
+// tile. Each CTA multiplies its eighth of k (u = x A^T, partial), the partial sums meet in distributed shared memory (each
+// CTA adds up an eighth of the tile's rows, in rank order, and stores them into all eight), and each CTA multiplies u by
+// its eighth of the columns of B and adds y. Both products are m16n8k16 matrix instructions fed straight from global
+// memory: the contraction index may be taken in any order as long as both operands agree, so a lane loads eight
+// consecutive values (16 bytes) of a row and uses them as the fragments of two instructions, and no operand passes
+// through shared memory but u.
+//
+// The sum over k has one order for every batch: k in blocks of 32, block j of a CTA in chain j mod 8, a chain's blocks one
+// after another in an accumulator of its own, chains added in order, then the eight CTAs' sums in rank order. So a row's
+// bits do not depend on the tile's size or on the rows beside it.
 #include <cuda_runtime.h>
+
+#include <limits.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "host.hpp"
@@ -7,69 +23,441 @@
 namespace esp {
 namespace {
 
+constexpr int CTAS = 8, CHAINS = 8, THREADS = 256, WARPS = THREADS / 32, MAX_SLOTS = 4096;
+constexpr int NO_PLAN = 64;             // up to this many rows every CTA finds its tile's rows itself
+constexpr int GROUP = 8;                // n8 tiles of the first product that a warp holds at once
+
 struct AdaptParams {
     esp_adapters_t ad;
     const void *x, *y;
     const int* ids;
     void* out;
+    const int* plan;        // tiles, then rows (above NO_PLAN rows)
     long long x_stride, y_stride, out_stride;
-    int n;
+    int rows, n, max_tiles;
 };
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+// A tile of the plan: its adapter (-1: none), where its rows start in the list of rows, how many there are.
+struct Tile {
+    int slot, first, count, unused;
+};
 
-// A CTA a row: the rank products by a warp each, then a column a thread.
-template <typename T>
-__global__ void adapt_kernel(AdaptParams p) {
-    extern __shared__ float u[];        // [n_mats][rank]
+__device__ __forceinline__ int slot_of(const AdaptParams& p, int t) {
+    const int id = p.ids[t];
+    return id >= 0 && id < p.ad.slots ? id : -1;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// The plan: rows sorted by adapter and cut into tiles, by one CTA. Places within an adapter are taken by atomics, so the
+// order of a tile's rows may change from run to run; no row's result depends on it.
+// ---------------------------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(1024) plan_kernel(AdaptParams p, Tile* tiles, int* rows, int m) {
+    extern __shared__ int count[];      // [slots + 1]: the rows of a slot, then where its next row goes; last: no adapter
+    __shared__ int warp_rows[32], warp_tiles[32], base_rows, base_tiles;
     pdl_launch_dependents();
     pdl_wait();
-    const int t = blockIdx.x, slot = p.ids[t], lane = threadIdx.x & 31, cap = p.ad.rank, K = p.ad.k;
-    const T* x = static_cast<const T*>(p.x) + t * p.x_stride;
-    const T* y = static_cast<const T*>(p.y) + t * p.y_stride;
-    T* out = static_cast<T*>(p.out) + t * p.out_stride;
-    int rank = 0;
-    if (slot >= 0 && slot < p.ad.slots) rank = p.ad.ranks ? min(max(p.ad.ranks[slot], 0), cap) : cap;
-    const float scale = rank && p.ad.scales ? p.ad.scales[slot] : 1.0f;
-    for (int j = threadIdx.x >> 5; j < p.ad.n_mats * cap; j += blockDim.x >> 5) {
-        if (j % cap >= rank) continue;
-        const T* a = static_cast<const T*>(p.ad.a) + (static_cast<size_t>(slot) * p.ad.n_mats * cap + j) * K;
-        float s = 0.0f;
-        for (int i = lane; i < K; i += 32) s = fmaf(to_f32(x[i]), to_f32(a[i]), s);
-#pragma unroll
-        for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-        if (lane == 0) u[j] = s;
+    const int slots = p.ad.slots + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int s = tid; s < slots; s += 1024) count[s] = 0;
+    if (tid == 0) base_rows = base_tiles = 0;
+    __syncthreads();
+    for (int t0 = 0; t0 < p.rows; t0 += 1024) {
+        const int t = t0 + tid, id = t < p.rows ? slot_of(p, t) : -2;
+        const unsigned same = __match_any_sync(0xffffffffu, id);
+        if (id >= -1 && lane == __ffs(same) - 1) atomicAdd(&count[id < 0 ? slots - 1 : id], __popc(same));
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < p.n; c += blockDim.x) {
-        float s = 0.0f;
-        if (rank) {
-            int m = 0;
-            for (int edge = p.ad.widths[0]; c >= edge; edge += p.ad.widths[++m]) {}
-            const T* b = static_cast<const T*>(p.ad.b) + (static_cast<size_t>(slot) * p.n + c) * cap;
-            for (int j = 0; j < rank; ++j) s = fmaf(u[m * cap + j], to_f32(b[j]), s);
+    // exclusive sums over the slots of their rows and tiles, 1024 slots a round
+    for (int s0 = 0; s0 < slots; s0 += 1024) {
+        const int s = s0 + tid, c = s < slots ? count[s] : 0, n = (c + m - 1) / m;
+        int sum_c = c, sum_n = n;
+#pragma unroll
+        for (int k = 1; k < 32; k <<= 1) {
+            const int a = __shfl_up_sync(0xffffffffu, sum_c, k), b = __shfl_up_sync(0xffffffffu, sum_n, k);
+            if (lane >= k) sum_c += a, sum_n += b;
         }
-        out[c] = rank ? from_f32<T>(fmaf(scale, s, to_f32(y[c]))) : y[c];
+        if (lane == 31) warp_rows[warp] = sum_c, warp_tiles[warp] = sum_n;
+        __syncthreads();
+        if (warp == 0) {
+            int a = warp_rows[lane], b = warp_tiles[lane];
+#pragma unroll
+            for (int k = 1; k < 32; k <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, a, k), v = __shfl_up_sync(0xffffffffu, b, k);
+                if (lane >= k) a += u, b += v;
+            }
+            warp_rows[lane] = a, warp_tiles[lane] = b;
+        }
+        __syncthreads();
+        const int at = base_rows + sum_c - c + (warp ? warp_rows[warp - 1] : 0);
+        const int tile = base_tiles + sum_n - n + (warp ? warp_tiles[warp - 1] : 0);
+        for (int i = 0; i < n; ++i)
+            tiles[tile + i] = {s == slots - 1 ? -1 : s, at + i * m, min(m, c - i * m), 0};
+        if (s < slots) count[s] = at;
+        __syncthreads();
+        if (tid == 0) base_rows += warp_rows[31], base_tiles += warp_tiles[31];
+        __syncthreads();
+    }
+    for (int i = base_tiles + tid; i < p.max_tiles; i += 1024) tiles[i] = {-1, 0, 0, 0};
+    for (int t0 = 0; t0 < p.rows; t0 += 1024) {
+        const int t = t0 + tid, id = t < p.rows ? slot_of(p, t) : -2;
+        const unsigned same = __match_any_sync(0xffffffffu, id);
+        const int leader = __ffs(same) - 1;
+        int at = 0;
+        if (id >= -1 && lane == leader) at = atomicAdd(&count[id < 0 ? slots - 1 : id], __popc(same));
+        at = __shfl_sync(0xffffffffu, at, leader);
+        if (id >= -1) rows[at + __popc(same & ((1u << lane) - 1))] = t;
     }
 }
 
-constexpr int MAX_SLOTS = 4096;
+// ---------------------------------------------------------------------------------------------------------------
+// Matrix fragments
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float2 unpack(uint32_t v, __half) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+__device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) {
+    return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+}
+__device__ __forceinline__ uint32_t pack(float a, float b, __half) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// The product. ROW_WARPS x 16 rows a tile; RANK16 = the capacity in steps of 16. With one row warp the CTA's eight warps
+// take a chain each; with more, a warp has 16 rows and walks all chains, the remaining warps sharing the columns.
+// ---------------------------------------------------------------------------------------------------------------
+template <int ROW_WARPS>
+struct Shape {
+    static constexpr int M = 16 * ROW_WARPS;
+    static constexpr int COL_WARPS = WARPS / ROW_WARPS;     // warps that share a row group's columns
+};
+
+// Shared memory: sums [M][cols] fp32, u_hi and u_lo [M][stride] 16-bit (stride: cols + 8, so that rows start in other
+// banks), the rows' factors, and with one row warp the chains' sums [CHAINS][16][GROUP * 8].
+__host__ __device__ constexpr int u_stride(int cols) { return cols + 8; }
+template <int ROW_WARPS>
+size_t smem_bytes(int cols) {
+    const size_t m = Shape<ROW_WARPS>::M;
+    return m * cols * 4 + 2 * m * u_stride(cols) * 2 + m * 8 + (ROW_WARPS == 1 ? CHAINS * 16 * GROUP * 8 * 4 : 0);
+}
+
+template <typename T, int ROW_WARPS, int RANK16>
+__global__ void __launch_bounds__(THREADS, 2) adapt_kernel(AdaptParams p) {
+    constexpr int M = Shape<ROW_WARPS>::M, COL_WARPS = Shape<ROW_WARPS>::COL_WARPS, RP = RANK16 * 16;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ int tile_rows[M];
+    __shared__ int tile_slot, tile_count, found[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    const int rank = blockIdx.x % CTAS, tile = blockIdx.x / CTAS;
+    const int cap = p.ad.rank, K = p.ad.k, mats = p.ad.n_mats, cols = mats * RP, us = u_stride(cols);
+    float* sums = reinterpret_cast<float*>(smem);
+    T* u_hi = reinterpret_cast<T*>(sums + M * cols);
+    T* u_lo = u_hi + M * us;
+    float* factor = reinterpret_cast<float*>(u_lo + M * us);
+    float* chains = factor + 2 * M;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // The tile's adapter and rows.
+    if (p.plan) {
+        const Tile mine = reinterpret_cast<const Tile*>(p.plan)[tile];
+        if (mine.count == 0) return;        // (the whole cluster: one tile)
+        const int* rows = p.plan + 4 * p.max_tiles + mine.first;
+        for (int i = tid; i < M; i += THREADS) tile_rows[i] = i < mine.count ? rows[i] : -1;
+        if (tid == 0) tile_slot = mine.slot, tile_count = mine.count;
+    } else {
+        // Tile j is row j's if the rows of its adapter before it fill whole tiles; it takes the next M of them.
+        const int slot = slot_of(p, tile);
+        for (int i = tid; i < M; i += THREADS) tile_rows[i] = -1;
+        if (tid == 0) tile_slot = slot;
+        __syncthreads();
+        if (warp == 0) {
+            int before = 0, taken = 0;
+            for (int t0 = 0; t0 < p.rows; t0 += 32) {
+                const int t = t0 + lane;
+                const unsigned same = __ballot_sync(0xffffffffu, t < p.rows && slot_of(p, t) == slot);
+                const unsigned from = tile <= t0 ? 0xffffffffu : tile >= t0 + 32 ? 0u : ~0u << (tile - t0);
+                before += __popc(same & ~from);
+                const int at = taken + __popc(same & from & ((1u << lane) - 1));
+                if ((same & from) >> lane & 1 && at < M) tile_rows[at] = t;
+                taken += __popc(same & from);
+            }
+            if (lane == 0) tile_count = min(taken, M), found[0] = before % M == 0;
+        }
+        __syncthreads();
+        if (!found[0]) return;
+    }
+    __syncthreads();
+    const int slot = tile_slot, count = tile_count;
+    int r8 = 0;             // the adapter's rank, in whole steps of 8
+    if (slot >= 0) r8 = p.ad.ranks ? (min(max(p.ad.ranks[slot], 0), cap) + 7) / 8 * 8 : cap;
+    const T* x = static_cast<const T*>(p.x);
+    const T* y = static_cast<const T*>(p.y);
+    T* out = static_cast<T*>(p.out);
+
+    // this CTA's 32-column blocks of the output, matrix by matrix
+    int blocks = 0;
+    for (int m = 0; m < mats; ++m) blocks += (p.ad.widths[m] + 31) / 32;
+    const int block_lo = blocks * rank / CTAS, block_hi = blocks * (rank + 1) / CTAS;
+
+    if (r8 == 0) {          // nothing to add: y itself
+        if (out == y && p.out_stride == p.y_stride) return;
+        const int from = p.n / 8 * rank / CTAS, to = p.n / 8 * (rank + 1) / CTAS;
+        for (int r = warp; r < count; r += WARPS)
+            for (int c = from + lane; c < to; c += 32)
+                reinterpret_cast<uint4*>(out + tile_rows[r] * p.out_stride)[c] =
+                    reinterpret_cast<const uint4*>(y + tile_rows[r] * p.y_stride)[c];
+        return;
+    }
+
+    // u = x A^T over this CTA's blocks of k, GROUP n8 tiles at a time. Tile j of a matrix is its ranks 8 j .. 8 j + 7.
+    const int k_blocks = (K + 31) / 32, k_lo = k_blocks * rank / CTAS, k_hi = k_blocks * (rank + 1) / CTAS;
+    const int tiles_a_mat = r8 / 8, n_tiles = mats * tiles_a_mat;
+    const T* A = static_cast<const T*>(p.ad.a) + static_cast<size_t>(slot) * mats * cap * K;
+    const int row_warp = ROW_WARPS == 1 ? 0 : warp % ROW_WARPS, col_warp = ROW_WARPS == 1 ? 0 : warp / ROW_WARPS;
+    const int ra = tile_rows[row_warp * 16 + g], rb = tile_rows[row_warp * 16 + g + 8];
+    const T* xa = ra >= 0 ? x + ra * p.x_stride : nullptr;
+    const T* xb = rb >= 0 ? x + rb * p.x_stride : nullptr;
+    const uint4 zero = {0, 0, 0, 0};
+    const int per = ROW_WARPS == 1 ? GROUP : min(GROUP, (n_tiles + COL_WARPS - 1) / COL_WARPS);
+    const int groups = (n_tiles + per - 1) / per;
+    for (int gi = ROW_WARPS == 1 ? 0 : col_warp; gi < groups; gi += ROW_WARPS == 1 ? 1 : COL_WARPS) {
+        const int t0 = gi * per, nt = min(per, n_tiles - t0);
+        const T* a_row[GROUP];
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) {
+            const int t = min(t0 + j, n_tiles - 1), m = t / tiles_a_mat;
+            a_row[j] = A + (static_cast<size_t>(m) * cap + (t - m * tiles_a_mat) * 8 + g) * K;
+        }
+        float total[GROUP][4] = {};
+        for (int c = ROW_WARPS == 1 ? warp : 0; c < CHAINS; c += ROW_WARPS == 1 ? CHAINS : 1) {
+            float acc[GROUP][4] = {};
+            for (int kb = k_lo + c; kb < k_hi; kb += CHAINS) {
+                const int k = kb * 32 + q * 8;
+                const bool in = k < K;
+                const uint4 va = in && xa ? *reinterpret_cast<const uint4*>(xa + k) : zero;
+                const uint4 vb = in && xb ? *reinterpret_cast<const uint4*>(xb + k) : zero;
+                uint4 w[GROUP];
+#pragma unroll
+                for (int j = 0; j < GROUP; ++j)
+                    w[j] = in && j < nt ? *reinterpret_cast<const uint4*>(a_row[j] + k) : zero;
+                const uint32_t a0[4] = {va.x, vb.x, va.y, vb.y}, a1[4] = {va.z, vb.z, va.w, vb.w};
+#pragma unroll
+                for (int j = 0; j < GROUP; ++j)
+                    if (j < nt) {
+                        mma<T>(acc[j], a0, w[j].x, w[j].y);
+                        mma<T>(acc[j], a1, w[j].z, w[j].w);
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) total[j][e] += acc[j][e];
+        }
+        const auto column = [&](int t) {
+            const int m = t / tiles_a_mat;
+            return m * RP + (t - m * tiles_a_mat) * 8;
+        };
+        if constexpr (ROW_WARPS == 1) {
+            // chains[chain][row][GROUP * 8], then their sum in order
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j)
+                if (j < nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        chains[(warp * 16 + g + (e >> 1) * 8) * GROUP * 8 + j * 8 + q * 2 + (e & 1)] = total[j][e];
+            __syncthreads();
+            for (int i = tid; i < 16 * nt * 8; i += THREADS) {
+                const int r = i / (nt * 8), c = i - r * nt * 8;
+                float s = 0.0f;
+#pragma unroll
+                for (int w = 0; w < CHAINS; ++w) s += chains[(w * 16 + r) * GROUP * 8 + c];
+                sums[r * cols + column(t0 + c / 8) + c % 8] = s;
+            }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j)
+                if (j < nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sums[(row_warp * 16 + g + (e >> 1) * 8) * cols + column(t0 + j) + q * 2 + (e & 1)] = total[j][e];
+        }
+    }
+    cluster_sync_all();
+
+    // Add up the eight CTAs' sums of this CTA's eighth of the rows, in rank order, and store them into all eight as two
+    // 16-bit halves (hi + lo is the sum to 2^-16 of it, so the second product rounds nothing that the output shows). For
+    // fp16 a row is first scaled by a power of two that brings its largest value to [2^14, 2^15); the factor comes back
+    // with the adapter's scale.
+    const float scale = p.ad.scales ? p.ad.scales[slot] : 1.0f;
+    for (int r = rank * (M / CTAS) + warp; r < (rank + 1) * (M / CTAS); r += WARPS) {
+        float2 v[RANK16];
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < RANK16; ++i) {
+            const int c = lane * 2 + i * 64;
+            v[i] = {0.0f, 0.0f};
+            if (c < cols && c % RP < r8)
+#pragma unroll
+                for (int w = 0; w < CTAS; ++w) {
+                    const float2 o = ld_cluster_f2(sums + r * cols + c, w);
+                    v[i].x += o.x, v[i].y += o.y;
+                }
+            top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+        }
+        float up = 1.0f, down = scale;
+        if constexpr (std::is_same_v<T, __half>) {
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+            if (top > 1e-30f && top < 1e30f) {
+                const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
+                up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                down = scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RANK16; ++i) {
+            const int c = lane * 2 + i * 64;
+            if (c >= cols) continue;
+            const float a = v[i].x * up, b = v[i].y * up;
+            const uint32_t hi = pack(a, b, T());
+            const float2 back = unpack(hi, T());
+            // (an infinite half leaves nothing to the other one)
+            const uint32_t lo = pack(isinf(back.x) ? 0.0f : a - back.x, isinf(back.y) ? 0.0f : b - back.y, T());
+#pragma unroll
+            for (int w = 0; w < CTAS; ++w) {
+                st_cluster_u32(u_hi + r * us + c, w, hi);
+                st_cluster_u32(u_lo + r * us + c, w, lo);
+            }
+        }
+        if (lane < CTAS) st_cluster_u32(factor + r, lane, __float_as_uint(down));
+    }
+    cluster_sync_all();     // (the last access to another CTA's memory was before it)
+
+    // out = y + factor u B^T over this CTA's blocks of columns. The four n8 tiles of a block take columns so that a lane ends
+    // up with eight consecutive ones: tile j's column c is 8 (c / 2) + 2 j + c % 2 of the block.
+    const T* B = static_cast<const T*>(p.ad.b) + static_cast<size_t>(slot) * p.n * cap;
+    const float fa = factor[row_warp * 16 + g], fb = factor[row_warp * 16 + g + 8];
+    uint32_t hi[RANK16][4], lo[RANK16][4];
+    int m = -1, m_block = 0, m_col = 0, next_block = 0;       // the matrix of the block, its first block and column
+    for (int b = block_lo + (ROW_WARPS == 1 ? warp : col_warp); b < block_hi; b += ROW_WARPS == 1 ? WARPS : COL_WARPS) {
+        if (b >= next_block) {
+            while (b >= next_block) {
+                if (m >= 0) m_col += p.ad.widths[m];
+                m_block = next_block;
+                next_block += (p.ad.widths[++m] + 31) / 32;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const T* u = (h ? u_lo : u_hi) + (row_warp * 16 + g) * us + m * RP;
+                auto& f = h ? lo : hi;
+                if constexpr (RANK16 == 1) {
+                    const uint2 va = *reinterpret_cast<const uint2*>(u + q * 4);
+                    const uint2 vb = *reinterpret_cast<const uint2*>(u + 8 * us + q * 4);
+                    f[0][0] = va.x, f[0][1] = vb.x, f[0][2] = va.y, f[0][3] = vb.y;
+                } else {
+#pragma unroll
+                    for (int s = 0; s < RANK16; s += 2) {
+                        const uint4 va = *reinterpret_cast<const uint4*>(u + s * 16 + q * 8);
+                        const uint4 vb = *reinterpret_cast<const uint4*>(u + 8 * us + s * 16 + q * 8);
+                        f[s][0] = va.x, f[s][1] = vb.x, f[s][2] = va.y, f[s][3] = vb.y;
+                        f[s + 1][0] = va.z, f[s + 1][1] = vb.z, f[s + 1][2] = va.w, f[s + 1][3] = vb.w;
+                    }
+                }
+            }
+        }
+        const int width = p.ad.widths[m], base = (b - m_block) * 32;      // columns of matrix m
+        const bool in = base + q * 8 < width;
+        const int col = m_col + base + q * 8;
+        const uint4 ya = in && ra >= 0 ? *reinterpret_cast<const uint4*>(y + ra * p.y_stride + col) : zero;
+        const uint4 yb = in && rb >= 0 ? *reinterpret_cast<const uint4*>(y + rb * p.y_stride + col) : zero;
+        const bool n_in = base + (g >> 1) * 8 < width;
+        const T* w = B + (static_cast<size_t>(m_col) + base + (g >> 1) * 8 + (g & 1)) * cap;
+        float acc[4][4] = {};
+        if constexpr (RANK16 == 1) {
+            uint2 k[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                k[j] = n_in && q * 4 < r8 ? *reinterpret_cast<const uint2*>(w + j * 2 * cap + q * 4) : uint2{0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                mma<T>(acc[j], hi[0], k[j].x, k[j].y);
+                mma<T>(acc[j], lo[0], k[j].x, k[j].y);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < RANK16; s += 2) {
+                if (s * 16 >= r8) break;
+                uint4 k[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    k[j] = n_in && s * 16 + q * 8 < r8 ? *reinterpret_cast<const uint4*>(w + j * 2 * cap + s * 16 + q * 8)
+                                                       : zero;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    mma<T>(acc[j], hi[s], k[j].x, k[j].y);
+                    mma<T>(acc[j], lo[s], k[j].x, k[j].y);
+                    mma<T>(acc[j], hi[s + 1], k[j].z, k[j].w);
+                    mma<T>(acc[j], lo[s + 1], k[j].z, k[j].w);
+                }
+            }
+        }
+        if (!in) continue;
+        const auto add = [&](const uint4& v, int e, float f) {
+            uint4 o;
+            const uint32_t* from = &v.x;
+            uint32_t* to = &o.x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 b2 = unpack(from[j], T());
+                to[j] = pack(fmaf(f, acc[j][e], b2.x), fmaf(f, acc[j][e + 1], b2.y), T());
+            }
+            return o;
+        };
+        if (ra >= 0) *reinterpret_cast<uint4*>(out + ra * p.out_stride + col) = add(ya, 0, fa);
+        if (rb >= 0) *reinterpret_cast<uint4*>(out + rb * p.out_stride + col) = add(yb, 2, fb);
+    }
+}
+
+using Kernel = void (*)(AdaptParams);
+
+template <typename T, int ROW_WARPS>
+Kernel kernel_of(int rank16) {
+    return rank16 == 1   ? adapt_kernel<T, ROW_WARPS, 1>
+           : rank16 == 2 ? adapt_kernel<T, ROW_WARPS, 2>
+           : rank16 == 4 ? adapt_kernel<T, ROW_WARPS, 4>
+                         : adapt_kernel<T, ROW_WARPS, 8>;
+}
+
+int rank_steps(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
+
+// Tiles a plan may need: every adapter's rows (and those without one) end with a tile that is not full.
+long long max_tiles(int rows, int slots, int m) { return (rows + m - 1) / m + (rows < slots + 1 ? rows : slots + 1); }
 
 }  // namespace
 }  // namespace esp
 
-extern "C" size_t esp_adapt_ws_bytes(int, int) { return 0; }
+extern "C" size_t esp_adapt_ws_bytes(int t_rows, int slots) {
+    using namespace esp;
+    if (t_rows <= NO_PLAN || slots < 1) return 0;
+    return static_cast<size_t>(max_tiles(t_rows, slots, 16)) * sizeof(Tile) + static_cast<size_t>(t_rows) * sizeof(int);
+}
 
 extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_stride, const void* y, long long y_stride,
                          const int* ids, int t_rows, void* out, long long out_stride, void* ws, size_t ws_bytes,
@@ -88,8 +476,8 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
                     "esp_adapt: width %d is not a multiple of 8", ad->widths[m]);
         n += ad->widths[m];
     }
-    ESP_REQUIRE(n < (1ll << 31), ESP_ERR_INVALID, "esp_adapt: %lld columns", n);
-    ESP_REQUIRE(t_rows >= 0, ESP_ERR_INVALID, "esp_adapt: %d rows", t_rows);
+    ESP_REQUIRE(n < INT_MAX - 128, ESP_ERR_INVALID, "esp_adapt: %lld columns", n);
+    ESP_REQUIRE(t_rows >= 0 && t_rows <= (1 << 26), ESP_ERR_INVALID, "esp_adapt: %d rows", t_rows);
     if (t_rows == 0) return ok();
     ESP_REQUIRE(ad->a && ad->b && x && y && ids && out, ESP_ERR_INVALID, "esp_adapt: null pointer");
     ESP_REQUIRE(aligned(ad->a, 16) && aligned(ad->b, 16) && aligned(x, 16) && aligned(y, 16) && aligned(out, 16) &&
@@ -98,9 +486,27 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
     const size_t need = esp_adapt_ws_bytes(t_rows, ad->slots);
     ESP_REQUIRE(need == 0 || (ws && aligned(ws, 16) && ws_bytes >= need), ESP_ERR_SCRATCH,
                 "esp_adapt: workspace of %zu bytes, %zu needed (16-byte aligned)", ws ? ws_bytes : 0, need);
-    const AdaptParams p{*ad, x, y, ids, out, x_stride, y_stride, out_stride, static_cast<int>(n)};
-    const auto kernel = ad->dtype == F16 ? adapt_kernel<__half> : adapt_kernel<__nv_bfloat16>;
-    if (const int rc = launch(kernel, dim3(t_rows), dim3(256), sizeof(float) * ad->n_mats * ad->rank, stream, true, p))
+
+    const int steps = rank_steps(ad->rank), cols = ad->n_mats * steps * 16;
+    const bool half = ad->dtype == F16;
+    // Tiles of 64 rows where adapters have that many on average and their shared memory lets two CTAs on an SM.
+    const bool wide = t_rows > NO_PLAN && t_rows / ad->slots >= 32 && cols <= 192;
+    const int m = wide ? 64 : 16;
+    const size_t smem = wide ? smem_bytes<4>(cols) : smem_bytes<1>(cols);
+    const Kernel kernel = wide ? (half ? kernel_of<__half, 4>(steps) : kernel_of<__nv_bfloat16, 4>(steps))
+                               : (half ? kernel_of<__half, 1>(steps) : kernel_of<__nv_bfloat16, 1>(steps));
+    AdaptParams p{*ad, x, y, ids, out, nullptr, x_stride, y_stride, out_stride, t_rows, static_cast<int>(n), t_rows};
+    if (t_rows > NO_PLAN) {
+        p.max_tiles = static_cast<int>(max_tiles(t_rows, ad->slots, m));
+        Tile* tiles = static_cast<Tile*>(ws);
+        p.plan = static_cast<const int*>(ws);
+        if (const int rc = launch(plan_kernel, dim3(1), dim3(1024), sizeof(int) * (ad->slots + 1), stream, true, p, tiles,
+                                  reinterpret_cast<int*>(tiles + p.max_tiles), m))
+            return rc;
+    }
+    if (const int rc = allow_smem(kernel, smem)) return rc;
+    if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * CTAS), dim3(THREADS), smem, stream,
+                                      true, CTAS, p))
         return rc;
     return ok();
 }

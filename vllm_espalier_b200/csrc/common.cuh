@@ -194,6 +194,19 @@ __device__ __forceinline__ float4 ld_cluster_f4(const void* local, uint32_t rank
     return v;
 }
 
+__device__ __forceinline__ float2 ld_cluster_f2(const void* local, uint32_t rank) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(local)), "r"(rank));
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_cluster_u32(void* local, uint32_t rank, uint32_t v) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(local)), "r"(rank));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
+}
+
 // Four words into another CTA's shared memory, their 16 bytes counted on an mbarrier there (both given by this CTA's own
 // addresses of the same objects): who waits for the barrier's bytes sees the words, with no barrier of the cluster.
 __device__ __forceinline__ void st_async_v4(void* local, uint64_t* bar, uint32_t rank, uint32_t a, uint32_t b, uint32_t c,

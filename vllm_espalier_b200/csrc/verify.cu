@@ -34,7 +34,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, PACKS = 4, OCTETS = 2, SINGLES = 8, RESIDENT = 4;
-constexpr int MAX_SEGMENTS = 16, SEGMENT = 16384, FILL = 1000;
+constexpr int MAX_SEGMENTS = 16, SEGMENT = 16384, FILL = 4;
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float rcp(float x) {
