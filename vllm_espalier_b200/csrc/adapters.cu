@@ -8,13 +8,13 @@
 // consecutive values (16 bytes) of a row and uses them as the fragments of two instructions, and no operand passes
 // through shared memory but u.
 //
-// The sum over k has one order for every batch: k in blocks of 32, block j of a CTA in chain j mod 8, a chain's blocks one
-// after another in an accumulator of its own, chains added in order, then the eight CTAs' sums in rank order. So a row's
-// bits do not depend on the tile's size or on the rows beside it.
+// The sum over k has one order for every batch: a CTA's share of k in ascending order in one accumulator, then the eight
+// CTAs' sums in rank order. So a row's bits do not depend on the tile's size or on the rows beside it.
 #include <cuda_runtime.h>
 
 #include <limits.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -23,9 +23,8 @@
 namespace esp {
 namespace {
 
-constexpr int CTAS = 8, CHAINS = 8, THREADS = 256, WARPS = THREADS / 32, MAX_SLOTS = 4096;
+constexpr int CTAS = 8, MAX_SLOTS = 4096;
 constexpr int NO_PLAN = 64;             // up to this many rows every CTA finds its tile's rows itself
-constexpr int GROUP = 8;                // n8 tiles of the first product that a warp holds at once
 
 struct AdaptParams {
     esp_adapters_t ad;
@@ -139,27 +138,37 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// The product. ROW_WARPS x 16 rows a tile; RANK16 = the capacity in steps of 16. With one row warp the CTA's eight warps
-// take a chain each; with more, a warp has 16 rows and walks all chains, the remaining warps sharing the columns.
+// The product: tiles of M = 16 ROW_WARPS rows, RANK16 = the capacity in steps of 16.
+//   ROW_WARPS 1 (few rows an adapter): eight warps share the inner columns, operands straight from global memory, the
+//   loads of many blocks of k asked for before the first product.
+//   ROW_WARPS 4 (prefill): sixteen warps, four row groups by four shares of the columns, x and A through a ring of
+//   shared memory (16-byte asynchronous copies, STAGE_K values of k a stage), so that a CTA's whole share is on its way
+//   while the first stages are multiplied.
 // ---------------------------------------------------------------------------------------------------------------
 template <int ROW_WARPS>
 struct Shape {
     static constexpr int M = 16 * ROW_WARPS;
-    static constexpr int COL_WARPS = WARPS / ROW_WARPS;     // warps that share a row group's columns
+    static constexpr int COL_WARPS = ROW_WARPS == 1 ? 8 : 4;    // warps that share a row group's columns of the output
+    static constexpr int WARPS = ROW_WARPS * COL_WARPS, THREADS = 32 * WARPS;
+    static constexpr int GROUP = ROW_WARPS == 1 ? 3 : 6;        // n8 tiles of the first product that a warp holds at once
 };
+constexpr int STAGE_K = 64, MAX_STAGES = 4, WIDE_COLS = Shape<4>::GROUP * 8 * Shape<4>::COL_WARPS;
 
-// Shared memory: sums [M][cols] fp32, u_hi and u_lo [M][stride] 16-bit (stride: cols + 8, so that rows start in other
-// banks), the rows' factors, and with one row warp the chains' sums [CHAINS][16][GROUP * 8].
-__host__ __device__ constexpr int u_stride(int cols) { return cols + 8; }
+// Shared memory: sums [M][cols] fp32, u_hi and u_lo [M][stride] 16-bit (stride: 64 bytes past a multiple of 128, so that
+// the eight lanes of a quarter load meet every bank once), the rows' factors; with four row warps the same place holds the
+// ring before.
+__host__ __device__ constexpr int u_stride(int cols) { return cols + (192 - cols * 2 % 128) % 128 / 2; }
 template <int ROW_WARPS>
-size_t smem_bytes(int cols) {
-    const size_t m = Shape<ROW_WARPS>::M;
-    return m * cols * 4 + 2 * m * u_stride(cols) * 2 + m * 8 + (ROW_WARPS == 1 ? CHAINS * 16 * GROUP * 8 * 4 : 0);
+__host__ __device__ constexpr int joined_bytes(int cols) {
+    return Shape<ROW_WARPS>::M * (cols * 4 + 2 * u_stride(cols) * 2 + 8);
 }
+constexpr int stage_bytes(int cols) { return (Shape<4>::M + cols) * STAGE_K * 2; }
 
 template <typename T, int ROW_WARPS, int RANK16>
-__global__ void __launch_bounds__(THREADS, 2) adapt_kernel(AdaptParams p) {
-    constexpr int M = Shape<ROW_WARPS>::M, COL_WARPS = Shape<ROW_WARPS>::COL_WARPS, RP = RANK16 * 16;
+__global__ void __launch_bounds__(Shape<ROW_WARPS>::THREADS, 2) adapt_kernel(AdaptParams p, int stages) {
+    using S = Shape<ROW_WARPS>;
+    constexpr int M = S::M, COL_WARPS = S::COL_WARPS, WARPS = S::WARPS, THREADS = S::THREADS, GROUP = S::GROUP;
+    constexpr int RP = RANK16 * 16;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int tile_rows[M];
     __shared__ int tile_slot, tile_count, found[2];
@@ -170,7 +179,6 @@ __global__ void __launch_bounds__(THREADS, 2) adapt_kernel(AdaptParams p) {
     T* u_hi = reinterpret_cast<T*>(sums + M * cols);
     T* u_lo = u_hi + M * us;
     float* factor = reinterpret_cast<float*>(u_lo + M * us);
-    float* chains = factor + 2 * M;
     pdl_launch_dependents();
     pdl_wait();
 
@@ -226,79 +234,142 @@ __global__ void __launch_bounds__(THREADS, 2) adapt_kernel(AdaptParams p) {
         return;
     }
 
-    // u = x A^T over this CTA's blocks of k, GROUP n8 tiles at a time. Tile j of a matrix is its ranks 8 j .. 8 j + 7.
+    const T* B = static_cast<const T*>(p.ad.b) + static_cast<size_t>(slot) * p.n * cap;
+    {   // what the second product will read, into L2 meanwhile
+        int col_lo = p.n, col_hi = 0, first = 0, col = 0;
+        for (int m = 0; m < mats; ++m) {
+            const int w = p.ad.widths[m], n = (w + 31) / 32, from = max(block_lo - first, 0), to = min(block_hi - first, n);
+            if (from < to) col_lo = min(col_lo, col + from * 32), col_hi = max(col_hi, col + min(w, to * 32));
+            first += n, col += w;
+        }
+        if (col_lo < col_hi) {
+            if (tid < count) prefetch_l2(y + tile_rows[tid] * p.y_stride + col_lo, (col_hi - col_lo) * sizeof(T));
+            if (tid == THREADS - 1)
+                prefetch_l2(B + static_cast<size_t>(col_lo) * cap, static_cast<size_t>(col_hi - col_lo) * cap * sizeof(T));
+        }
+    }
+
+    // u = x A^T over this CTA's blocks of k. n8 tile t of the inner columns is ranks 8 j .. 8 j + 7 of matrix m, t = m
+    // (r8 / 8) + j.
     const int k_blocks = (K + 31) / 32, k_lo = k_blocks * rank / CTAS, k_hi = k_blocks * (rank + 1) / CTAS;
     const int tiles_a_mat = r8 / 8, n_tiles = mats * tiles_a_mat;
     const T* A = static_cast<const T*>(p.ad.a) + static_cast<size_t>(slot) * mats * cap * K;
-    const int row_warp = ROW_WARPS == 1 ? 0 : warp % ROW_WARPS, col_warp = ROW_WARPS == 1 ? 0 : warp / ROW_WARPS;
+    const int row_warp = ROW_WARPS == 1 ? 0 : warp % ROW_WARPS, col_warp = warp / ROW_WARPS;
     const int ra = tile_rows[row_warp * 16 + g], rb = tile_rows[row_warp * 16 + g + 8];
-    const T* xa = ra >= 0 ? x + ra * p.x_stride : nullptr;
-    const T* xb = rb >= 0 ? x + rb * p.x_stride : nullptr;
     const uint4 zero = {0, 0, 0, 0};
-    const int per = ROW_WARPS == 1 ? GROUP : min(GROUP, (n_tiles + COL_WARPS - 1) / COL_WARPS);
-    const int groups = (n_tiles + per - 1) / per;
-    for (int gi = ROW_WARPS == 1 ? 0 : col_warp; gi < groups; gi += ROW_WARPS == 1 ? 1 : COL_WARPS) {
-        const int t0 = gi * per, nt = min(per, n_tiles - t0);
-        const T* a_row[GROUP];
+    const auto a_row = [&](int t, int r) {      // row r of tile t of A
+        const int m = t / tiles_a_mat;
+        return A + (static_cast<size_t>(m) * cap + (t - m * tiles_a_mat) * 8 + r) * K;
+    };
+    const auto column = [&](int t) {            // its first column in sums and u
+        const int m = t / tiles_a_mat;
+        return m * RP + (t - m * tiles_a_mat) * 8;
+    };
+    if constexpr (ROW_WARPS == 1) {
+        const T* xa = ra >= 0 ? x + ra * p.x_stride : nullptr;
+        const T* xb = rb >= 0 ? x + rb * p.x_stride : nullptr;
+        // G tiles a warp at once (t0, t0 + WARPS, ...), U blocks of k asked for at once
+        const auto product = [&](auto G_, auto U_) {
+            constexpr int G = G_, U = U_;
+            for (int t0 = warp; t0 < n_tiles; t0 += G * WARPS) {
+                const T* from[G];
 #pragma unroll
-        for (int j = 0; j < GROUP; ++j) {
-            const int t = min(t0 + j, n_tiles - 1), m = t / tiles_a_mat;
-            a_row[j] = A + (static_cast<size_t>(m) * cap + (t - m * tiles_a_mat) * 8 + g) * K;
+                for (int j = 0; j < G; ++j) from[j] = t0 + j * WARPS < n_tiles ? a_row(t0 + j * WARPS, g) : nullptr;
+                float acc[G][4] = {};
+                for (int k0 = k_lo; k0 < k_hi; k0 += U) {
+                    uint4 va[U], vb[U], w[U][G];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int k = (k0 + u) * 32 + q * 8;
+                        const bool in = k0 + u < k_hi && k < K;
+                        va[u] = in && xa ? *reinterpret_cast<const uint4*>(xa + k) : zero;
+                        vb[u] = in && xb ? *reinterpret_cast<const uint4*>(xb + k) : zero;
+#pragma unroll
+                        for (int j = 0; j < G; ++j)
+                            w[u][j] = in && from[j] ? *reinterpret_cast<const uint4*>(from[j] + k) : zero;
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const uint32_t a0[4] = {va[u].x, vb[u].x, va[u].y, vb[u].y};
+                        const uint32_t a1[4] = {va[u].z, vb[u].z, va[u].w, vb[u].w};
+                        if (k0 + u < k_hi)
+#pragma unroll
+                            for (int j = 0; j < G; ++j) {
+                                mma<T>(acc[j], a0, w[u][j].x, w[u][j].y);
+                                mma<T>(acc[j], a1, w[u][j].z, w[u][j].w);
+                            }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < G; ++j)
+                    if (from[j])
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2)
+                            *reinterpret_cast<float2*>(&sums[(g + e * 4) * cols + column(t0 + j * WARPS) + q * 2]) =
+                                make_float2(acc[j][e], acc[j][e + 1]);
+            }
+        };
+        if (n_tiles <= WARPS) product(std::integral_constant<int, 1>(), std::integral_constant<int, 6>());
+        else product(std::integral_constant<int, GROUP>(), std::integral_constant<int, 4>());
+    } else {
+        // A stage: M rows of x, then the rows of A, 128 bytes each; 16-byte piece c of row r lies at c ^ 4 (r % 2), so that
+        // the eight lanes of a quarter load (two rows, four pieces) meet every bank once.
+        const int a_rows = n_tiles * 8, n_stages = ((k_hi - k_lo) * 32 + STAGE_K - 1) / STAGE_K;
+        const auto fill = [&](int i) {
+            unsigned char* to = smem + (i % stages) * stage_bytes(cols);
+            const int k0 = k_lo * 32 + i * STAGE_K;
+            for (int piece = tid; piece < (M + a_rows) * 8; piece += THREADS) {
+                const int r = piece >> 3, c = piece & 7, k = k0 + c * 8;
+                const T* from = nullptr;
+                if (k < k_hi * 32 && k < K) {
+                    if (r >= M) from = a_row((r - M) >> 3, (r - M) & 7) + k;
+                    else if (tile_rows[r] >= 0) from = x + tile_rows[r] * p.x_stride + k;
+                }
+                uint4* at = reinterpret_cast<uint4*>(to + r * 128 + (c ^ (r & 1) << 2) * 16);
+                if (from) cp_async16(at, from);
+                else *at = zero;
+            }
+        };
+        const int per = (n_tiles + COL_WARPS - 1) / COL_WARPS, t0 = col_warp * per, nt = min(per, n_tiles - t0);
+        float acc[GROUP][4] = {};
+        for (int i = 0; i < stages - 1; ++i) {
+            if (i < n_stages) fill(i);
+            cp_async_commit();
         }
-        float total[GROUP][4] = {};
-        for (int c = ROW_WARPS == 1 ? warp : 0; c < CHAINS; c += ROW_WARPS == 1 ? CHAINS : 1) {
-            float acc[GROUP][4] = {};
-            for (int kb = k_lo + c; kb < k_hi; kb += CHAINS) {
-                const int k = kb * 32 + q * 8;
-                const bool in = k < K;
-                const uint4 va = in && xa ? *reinterpret_cast<const uint4*>(xa + k) : zero;
-                const uint4 vb = in && xb ? *reinterpret_cast<const uint4*>(xb + k) : zero;
-                uint4 w[GROUP];
+        for (int i = 0; i < n_stages; ++i) {
+            if (stages == 4) cp_async_wait<2>();        // the stage after this and the one behind it may be on their way
+            else cp_async_wait<1>();
+            __syncthreads();
+            if (i + stages - 1 < n_stages) fill(i + stages - 1);
+            cp_async_commit();
+            const unsigned char* from = smem + (i % stages) * stage_bytes(cols);
 #pragma unroll
-                for (int j = 0; j < GROUP; ++j)
-                    w[j] = in && j < nt ? *reinterpret_cast<const uint4*>(a_row[j] + k) : zero;
+            for (int h = 0; h < STAGE_K / 32; ++h) {
+                const int kb = k_lo + i * (STAGE_K / 32) + h;
+                if (kb >= k_hi) break;
+                const auto piece = [&](int r) {
+                    return *reinterpret_cast<const uint4*>(from + r * 128 + ((h * 4 + q) ^ (r & 1) << 2) * 16);
+                };
+                const uint4 va = piece(row_warp * 16 + g), vb = piece(row_warp * 16 + g + 8);
                 const uint32_t a0[4] = {va.x, vb.x, va.y, vb.y}, a1[4] = {va.z, vb.z, va.w, vb.w};
 #pragma unroll
                 for (int j = 0; j < GROUP; ++j)
                     if (j < nt) {
-                        mma<T>(acc[j], a0, w[j].x, w[j].y);
-                        mma<T>(acc[j], a1, w[j].z, w[j].w);
+                        const uint4 w = piece(M + (t0 + j) * 8 + g);
+                        mma<T>(acc[j], a0, w.x, w.y);
+                        mma<T>(acc[j], a1, w.z, w.w);
                     }
             }
-#pragma unroll
-            for (int j = 0; j < GROUP; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) total[j][e] += acc[j][e];
         }
-        const auto column = [&](int t) {
-            const int m = t / tiles_a_mat;
-            return m * RP + (t - m * tiles_a_mat) * 8;
-        };
-        if constexpr (ROW_WARPS == 1) {
-            // chains[chain][row][GROUP * 8], then their sum in order
+        cp_async_wait<0>();
+        __syncthreads();        // the ring's place is free for the sums
 #pragma unroll
-            for (int j = 0; j < GROUP; ++j)
-                if (j < nt)
+        for (int j = 0; j < GROUP; ++j)
+            if (j < nt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        chains[(warp * 16 + g + (e >> 1) * 8) * GROUP * 8 + j * 8 + q * 2 + (e & 1)] = total[j][e];
-            __syncthreads();
-            for (int i = tid; i < 16 * nt * 8; i += THREADS) {
-                const int r = i / (nt * 8), c = i - r * nt * 8;
-                float s = 0.0f;
-#pragma unroll
-                for (int w = 0; w < CHAINS; ++w) s += chains[(w * 16 + r) * GROUP * 8 + c];
-                sums[r * cols + column(t0 + c / 8) + c % 8] = s;
-            }
-            __syncthreads();
-        } else {
-#pragma unroll
-            for (int j = 0; j < GROUP; ++j)
-                if (j < nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        sums[(row_warp * 16 + g + (e >> 1) * 8) * cols + column(t0 + j) + q * 2 + (e & 1)] = total[j][e];
-        }
+                for (int e = 0; e < 4; e += 2)
+                    *reinterpret_cast<float2*>(&sums[(row_warp * 16 + g + e * 4) * cols + column(t0 + j) + q * 2]) =
+                        make_float2(acc[j][e], acc[j][e + 1]);
     }
     cluster_sync_all();
 
@@ -352,35 +423,29 @@ __global__ void __launch_bounds__(THREADS, 2) adapt_kernel(AdaptParams p) {
 
     // out = y + factor u B^T over this CTA's blocks of columns. The four n8 tiles of a block take columns so that a lane ends
     // up with eight consecutive ones: tile j's column c is 8 (c / 2) + 2 j + c % 2 of the block.
-    const T* B = static_cast<const T*>(p.ad.b) + static_cast<size_t>(slot) * p.n * cap;
     const float fa = factor[row_warp * 16 + g], fb = factor[row_warp * 16 + g + 8];
-    uint32_t hi[RANK16][4], lo[RANK16][4];
     int m = -1, m_block = 0, m_col = 0, next_block = 0;       // the matrix of the block, its first block and column
-    for (int b = block_lo + (ROW_WARPS == 1 ? warp : col_warp); b < block_hi; b += ROW_WARPS == 1 ? WARPS : COL_WARPS) {
+    const T *h_at = nullptr, *l_at = nullptr;                 // this lane's halves of u for that matrix
+    const auto halves = [&](const T* u, int s, uint32_t (&f)[2][4]) {       // the fragments of steps s and s + 1
+        if constexpr (RANK16 == 1) {
+            const uint2 va = *reinterpret_cast<const uint2*>(u + q * 4), vb = *reinterpret_cast<const uint2*>(u + 8 * us + q * 4);
+            f[0][0] = va.x, f[0][1] = vb.x, f[0][2] = va.y, f[0][3] = vb.y;
+        } else {
+            const uint4 va = *reinterpret_cast<const uint4*>(u + s * 16 + q * 8);
+            const uint4 vb = *reinterpret_cast<const uint4*>(u + 8 * us + s * 16 + q * 8);
+            f[0][0] = va.x, f[0][1] = vb.x, f[0][2] = va.y, f[0][3] = vb.y;
+            f[1][0] = va.z, f[1][1] = vb.z, f[1][2] = va.w, f[1][3] = vb.w;
+        }
+    };
+    for (int b = block_lo + col_warp; b < block_hi; b += COL_WARPS) {
         if (b >= next_block) {
             while (b >= next_block) {
                 if (m >= 0) m_col += p.ad.widths[m];
                 m_block = next_block;
                 next_block += (p.ad.widths[++m] + 31) / 32;
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const T* u = (h ? u_lo : u_hi) + (row_warp * 16 + g) * us + m * RP;
-                auto& f = h ? lo : hi;
-                if constexpr (RANK16 == 1) {
-                    const uint2 va = *reinterpret_cast<const uint2*>(u + q * 4);
-                    const uint2 vb = *reinterpret_cast<const uint2*>(u + 8 * us + q * 4);
-                    f[0][0] = va.x, f[0][1] = vb.x, f[0][2] = va.y, f[0][3] = vb.y;
-                } else {
-#pragma unroll
-                    for (int s = 0; s < RANK16; s += 2) {
-                        const uint4 va = *reinterpret_cast<const uint4*>(u + s * 16 + q * 8);
-                        const uint4 vb = *reinterpret_cast<const uint4*>(u + 8 * us + s * 16 + q * 8);
-                        f[s][0] = va.x, f[s][1] = vb.x, f[s][2] = va.y, f[s][3] = vb.y;
-                        f[s + 1][0] = va.z, f[s + 1][1] = vb.z, f[s + 1][2] = va.w, f[s + 1][3] = vb.w;
-                    }
-                }
-            }
+            h_at = u_hi + (row_warp * 16 + g) * us + m * RP;
+            l_at = u_lo + (row_warp * 16 + g) * us + m * RP;
         }
         const int width = p.ad.widths[m], base = (b - m_block) * 32;      // columns of matrix m
         const bool in = base + q * 8 < width;
@@ -390,11 +455,14 @@ __global__ void __launch_bounds__(THREADS, 2) adapt_kernel(AdaptParams p) {
         const bool n_in = base + (g >> 1) * 8 < width;
         const T* w = B + (static_cast<size_t>(m_col) + base + (g >> 1) * 8 + (g & 1)) * cap;
         float acc[4][4] = {};
+        uint32_t hi[2][4], lo[2][4];
         if constexpr (RANK16 == 1) {
             uint2 k[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 k[j] = n_in && q * 4 < r8 ? *reinterpret_cast<const uint2*>(w + j * 2 * cap + q * 4) : uint2{0, 0};
+            halves(h_at, 0, hi);
+            halves(l_at, 0, lo);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 mma<T>(acc[j], hi[0], k[j].x, k[j].y);
@@ -409,12 +477,14 @@ __global__ void __launch_bounds__(THREADS, 2) adapt_kernel(AdaptParams p) {
                 for (int j = 0; j < 4; ++j)
                     k[j] = n_in && s * 16 + q * 8 < r8 ? *reinterpret_cast<const uint4*>(w + j * 2 * cap + s * 16 + q * 8)
                                                        : zero;
+                halves(h_at, s, hi);
+                halves(l_at, s, lo);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    mma<T>(acc[j], hi[s], k[j].x, k[j].y);
-                    mma<T>(acc[j], lo[s], k[j].x, k[j].y);
-                    mma<T>(acc[j], hi[s + 1], k[j].z, k[j].w);
-                    mma<T>(acc[j], lo[s + 1], k[j].z, k[j].w);
+                    mma<T>(acc[j], hi[0], k[j].x, k[j].y);
+                    mma<T>(acc[j], lo[0], k[j].x, k[j].y);
+                    mma<T>(acc[j], hi[1], k[j].z, k[j].w);
+                    mma<T>(acc[j], lo[1], k[j].z, k[j].w);
                 }
             }
         }
@@ -435,7 +505,7 @@ __global__ void __launch_bounds__(THREADS, 2) adapt_kernel(AdaptParams p) {
     }
 }
 
-using Kernel = void (*)(AdaptParams);
+using Kernel = void (*)(AdaptParams, int);
 
 template <typename T, int ROW_WARPS>
 Kernel kernel_of(int rank16) {
@@ -490,9 +560,11 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
     const int steps = rank_steps(ad->rank), cols = ad->n_mats * steps * 16;
     const bool half = ad->dtype == F16;
     // Tiles of 64 rows where adapters have that many on average and their shared memory lets two CTAs on an SM.
-    const bool wide = t_rows > NO_PLAN && t_rows / ad->slots >= 32 && cols <= 192;
-    const int m = wide ? 64 : 16;
-    const size_t smem = wide ? smem_bytes<4>(cols) : smem_bytes<1>(cols);
+    const bool wide = t_rows > NO_PLAN && t_rows / ad->slots >= 32 && cols <= WIDE_COLS;
+    const int m = wide ? Shape<4>::M : Shape<1>::M, threads = wide ? Shape<4>::THREADS : Shape<1>::THREADS;
+    const int stages = MAX_STAGES * stage_bytes(cols) <= 100 * 1024 ? MAX_STAGES : 3;
+    const size_t smem = wide ? std::max(joined_bytes<4>(cols), stages * stage_bytes(cols))
+                             : joined_bytes<1>(cols);
     const Kernel kernel = wide ? (half ? kernel_of<__half, 4>(steps) : kernel_of<__nv_bfloat16, 4>(steps))
                                : (half ? kernel_of<__half, 1>(steps) : kernel_of<__nv_bfloat16, 1>(steps));
     AdaptParams p{*ad, x, y, ids, out, nullptr, x_stride, y_stride, out_stride, t_rows, static_cast<int>(n), t_rows};
@@ -505,8 +577,8 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
             return rc;
     }
     if (const int rc = allow_smem(kernel, smem)) return rc;
-    if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * CTAS), dim3(THREADS), smem, stream,
-                                      true, CTAS, p))
+    if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * CTAS), dim3(threads), smem, stream,
+                                      true, CTAS, p, stages))
         return rc;
     return ok();
 }

@@ -246,6 +246,22 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {       // all but this thread's last N groups have landed
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Asks for the whole 16-byte blocks of a range into L2 (a hint, 64 KB an instruction).
+__device__ __forceinline__ void prefetch_l2(const void* p, size_t bytes) {
+    uintptr_t a = (reinterpret_cast<uintptr_t>(p) + 15) / 16 * 16;
+    const uintptr_t end = (reinterpret_cast<uintptr_t>(p) + bytes) / 16 * 16;
+    for (; a < end; a += 65536) {
+        const uint32_t n = static_cast<uint32_t>(end - a < 65536 ? end - a : 65536);
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a), "r"(n) : "memory");
+    }
+}
+
 // 1-D bulk copy global -> this CTA's shared memory (the tensor memory accelerator, no tensor map), completing `bytes`
 // on the mbarrier's transaction count. Both addresses 16-byte aligned, bytes a multiple of 16. No multicast.
 __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {

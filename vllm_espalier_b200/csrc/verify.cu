@@ -314,16 +314,6 @@ __device__ __noinline__ Part careful_part(const T* row, Segments own, float c, E
     return all;
 }
 
-// Asks for the whole 16-byte blocks of a range into L2 (a hint: at most 64 KB an instruction's worth at a time).
-__device__ __forceinline__ void prefetch_l2(const void* p, size_t bytes) {
-    uintptr_t a = (reinterpret_cast<uintptr_t>(p) + 15) / 16 * 16;
-    const uintptr_t end = (reinterpret_cast<uintptr_t>(p) + bytes) / 16 * 16;
-    for (; a < end; a += 65536) {
-        const uint32_t n = static_cast<uint32_t>(end - a < 65536 ? end - a : 65536);
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a), "r"(n) : "memory");
-    }
-}
-
 struct NoProbs {};      // the drafter chose its token outright
 template <typename Q>
 __device__ __forceinline__ float draft_prob(const Q* q, long long i) {
