@@ -1,15 +1,14 @@
 // Low-rank adapters of many requests at once beside a shared projection.
 //
-// out[t] = y[t] + scale (x[t] A^T) B^T. Rows are grouped by adapter into tiles of M rows; a cluster of eight CTAs takes a
-// tile. Each CTA multiplies its eighth of k (u = x A^T, partial), the partial sums meet in distributed shared memory (each
-// CTA adds up an eighth of the tile's rows, in rank order, and stores them into all eight), and each CTA multiplies u by
-// its eighth of the columns of B and adds y. Both products are m16n8k16 matrix instructions fed straight from global
-// memory: the contraction index may be taken in any order as long as both operands agree, so a lane loads eight
-// consecutive values (16 bytes) of a row and uses them as the fragments of two instructions, and no operand passes
-// through shared memory but u.
+// out[t] = y[t] + scale (x[t] A^T) B^T. Rows are grouped by adapter into tiles; a cluster of CTAs takes a tile. Each CTA
+// multiplies its share of k (u = x A^T, partial), the partial sums meet in distributed shared memory (each CTA joins its
+// share of the tile's rows and stores them into all), and each CTA multiplies u by its share of the columns of B and adds y.
+// Both products are m16n8k16 matrix instructions. The contraction index may be taken in any order as long as both operands
+// agree, so a lane loads eight consecutive values (16 bytes) of a row and uses them as the fragments of two instructions.
 //
-// The sum over k has one order for every batch: a CTA's share of k in ascending order in one accumulator, then the eight
-// CTAs' sums in rank order. So a row's bits do not depend on the tile's size or on the rows beside it.
+// The sum over k has one order for every batch: eight segments of k, each in ascending order in one accumulator, joined as
+// a balanced tree ((0 + 1) + (2 + 3)) + ((4 + 5) + (6 + 7)), whichever CTA has which. So a row's bits do not depend on the
+// tile's size or on the rows beside it.
 #include <cuda_runtime.h>
 
 #include <limits.h>
@@ -23,7 +22,7 @@
 namespace esp {
 namespace {
 
-constexpr int CTAS = 8, MAX_SLOTS = 4096;
+constexpr int SEGMENTS = 8, MAX_SLOTS = 4096;
 constexpr int NO_PLAN = 64;             // up to this many rows every CTA finds its tile's rows itself
 
 struct AdaptParams {
@@ -138,47 +137,212 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// The product: tiles of M = 16 ROW_WARPS rows, RANK16 = the capacity in steps of 16.
-//   ROW_WARPS 1 (few rows an adapter): eight warps share the inner columns, operands straight from global memory, the
-//   loads of many blocks of k asked for before the first product.
-//   ROW_WARPS 4 (prefill): sixteen warps, four row groups by four shares of the columns, x and A through a ring of
-//   shared memory (16-byte asynchronous copies, STAGE_K values of k a stage), so that a CTA's whole share is on its way
-//   while the first stages are multiplied.
+// What both kernels below share. Inner columns of a tile: RP = 16 RANK16 a matrix (the capacity in steps of 16), u of all
+// matrices side by side.
 // ---------------------------------------------------------------------------------------------------------------
-template <int ROW_WARPS>
-struct Shape {
-    static constexpr int M = 16 * ROW_WARPS;
-    static constexpr int COL_WARPS = ROW_WARPS == 1 ? 8 : 4;    // warps that share a row group's columns of the output
-    static constexpr int WARPS = ROW_WARPS * COL_WARPS, THREADS = 32 * WARPS;
-    static constexpr int GROUP = ROW_WARPS == 1 ? 3 : 6;        // n8 tiles of the first product that a warp holds at once
-};
-constexpr int STAGE_K = 64, MAX_STAGES = 4, WIDE_COLS = Shape<4>::GROUP * 8 * Shape<4>::COL_WARPS;
-
-// Shared memory: sums [M][cols] fp32, u_hi and u_lo [M][stride] 16-bit (stride: 64 bytes past a multiple of 128, so that
-// the eight lanes of a quarter load meet every bank once), the rows' factors; with four row warps the same place holds the
-// ring before.
+// Elements between rows of u's halves: 64 bytes past a multiple of 128, so that the eight lanes of a quarter load meet
+// every bank once.
 __host__ __device__ constexpr int u_stride(int cols) { return cols + (192 - cols * 2 % 128) % 128 / 2; }
-template <int ROW_WARPS>
-__host__ __device__ constexpr int joined_bytes(int cols) {
-    return Shape<ROW_WARPS>::M * (cols * 4 + 2 * u_stride(cols) * 2 + 8);
-}
-constexpr int stage_bytes(int cols) { return (Shape<4>::M + cols) * STAGE_K * 2; }
 
-template <typename T, int ROW_WARPS, int RANK16>
-__global__ void __launch_bounds__(Shape<ROW_WARPS>::THREADS, 2) adapt_kernel(AdaptParams p, int stages) {
-    using S = Shape<ROW_WARPS>;
-    constexpr int M = S::M, COL_WARPS = S::COL_WARPS, WARPS = S::WARPS, THREADS = S::THREADS, GROUP = S::GROUP;
+// Shared memory of a tile: sums [M][cols] fp32 of this CTA, then u_hi and u_lo [M][stride] 16-bit and the rows' factors.
+template <typename T>
+struct Inner {
+    float* sums;
+    T *hi, *lo;
+    float* factor;
+    int cols, stride;
+    __device__ __forceinline__ Inner(unsigned char* at, int m, int cols_) : cols(cols_), stride(u_stride(cols_)) {
+        sums = reinterpret_cast<float*>(at);
+        hi = reinterpret_cast<T*>(sums + m * cols);
+        lo = hi + m * stride;
+        factor = reinterpret_cast<float*>(lo + m * stride);
+    }
+};
+constexpr int sums_bytes(int m, int cols) { return m * cols * 4; }
+constexpr int halves_bytes(int m, int cols) { return m * (2 * u_stride(cols) * 2 + 4); }
+
+// The adapter of a slot: its rank in whole steps of 8 (0: nothing to add), its matrices.
+template <typename T>
+struct Adapter {
+    const T *a, *b;
+    int r8, tiles_a_mat, n_tiles, cap, k;     // n8 tiles of inner columns: a matrix, all
+    __device__ __forceinline__ Adapter(const AdaptParams& p, int slot) : r8(0), cap(p.ad.rank), k(p.ad.k) {
+        if (slot >= 0) r8 = p.ad.ranks ? (min(max(p.ad.ranks[slot], 0), cap) + 7) / 8 * 8 : cap;
+        tiles_a_mat = r8 / 8, n_tiles = p.ad.n_mats * tiles_a_mat;
+        const size_t s = slot < 0 ? 0 : slot;
+        a = static_cast<const T*>(p.ad.a) + s * p.ad.n_mats * cap * k;
+        b = static_cast<const T*>(p.ad.b) + s * p.n * cap;
+    }
+    __device__ __forceinline__ const T* a_row(int t, int r) const {        // row r of tile t of A
+        const int m = t / tiles_a_mat;
+        return a + (static_cast<size_t>(m) * cap + (t - m * tiles_a_mat) * 8 + r) * k;
+    }
+    template <int RP>
+    __device__ __forceinline__ int column(int t) const {                   // the tile's first column in sums and u
+        const int m = t / tiles_a_mat;
+        return m * RP + (t - m * tiles_a_mat) * 8;
+    }
+};
+
+// A block of 32 columns of the output (never across matrices): its matrix, first column, and how many columns are left of
+// the matrix from there on.
+struct Block {
+    int m, col, left;
+};
+__device__ __forceinline__ Block block_at(const AdaptParams& p, int b) {
+    int col = 0;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        const int w = p.ad.widths[m], n = (w + 31) / 32;
+        if (m == p.ad.n_mats - 1 || b < n) return {m, col + b * 32, w - b * 32};
+        b -= n, col += w;
+    }
+    return {0, 0, 0};
+}
+__device__ __forceinline__ int block_count(const AdaptParams& p) {
+    int n = 0;
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+        if (m < p.ad.n_mats) n += (p.ad.widths[m] + 31) / 32;
+    return n;
+}
+
+__device__ __forceinline__ int segment_at(int blocks, int s) { return blocks * s / SEGMENTS; }     // its first block of 32 k
+
+// Rows without an adapter: y itself, this CTA's share of the columns.
+template <typename T>
+__device__ __forceinline__ void copy_rows(const AdaptParams& p, const int* tile_rows, int count, int rank, int ctas, int warps) {
+    if (p.out == p.y && p.out_stride == p.y_stride) return;
+    const int from = p.n / 8 * rank / ctas, to = p.n / 8 * (rank + 1) / ctas;
+    for (int r = threadIdx.x / 32; r < count; r += warps)
+        for (int c = from + threadIdx.x % 32; c < to; c += 32)
+            reinterpret_cast<uint4*>(static_cast<T*>(p.out) + tile_rows[r] * p.out_stride)[c] =
+                reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + tile_rows[r] * p.y_stride)[c];
+}
+
+// Join the cluster's sums of one row (a warp) as the tree over the segments and store it into every CTA as two 16-bit
+// halves (hi + lo is the sum to 2^-16 of it, so the second product rounds nothing that the output shows). For fp16 a row
+// is first scaled by a power of two that brings its largest value to [2^14, 2^15); the factor comes back with the
+// adapter's scale.
+template <typename T, int RANK16, int CTAS>
+__device__ __forceinline__ void join_row(const Inner<T>& u, int r, int r8, float scale) {
     constexpr int RP = RANK16 * 16;
-    extern __shared__ __align__(16) unsigned char smem[];
+    const int lane = threadIdx.x % 32;
+    float2 v[RANK16];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < RANK16; ++i) {
+        const int c = lane * 2 + i * 64;
+        v[i] = {0.0f, 0.0f};
+        if (c < u.cols && c % RP < r8) {
+            float2 o[CTAS];
+#pragma unroll
+            for (int w = 0; w < CTAS; ++w) o[w] = ld_cluster_f2(u.sums + r * u.cols + c, w);
+#pragma unroll
+            for (int n = 1; n < CTAS; n *= 2)
+#pragma unroll
+                for (int w = 0; w < CTAS; w += 2 * n) o[w].x += o[w + n].x, o[w].y += o[w + n].y;
+            v[i] = o[0];
+        }
+        top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+    }
+    float up = 1.0f, down = scale;
+    if constexpr (std::is_same_v<T, __half>) {
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+        if (top > 1e-30f && top < 1e30f) {
+            const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
+            up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            down = scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RANK16; ++i) {
+        const int c = lane * 2 + i * 64;
+        if (c >= u.cols) continue;
+        const float a = v[i].x * up, b = v[i].y * up;
+        const uint32_t hi = pack(a, b, T());
+        const float2 back = unpack(hi, T());
+        // (an infinite half leaves nothing to the other one)
+        const uint32_t lo = pack(isinf(back.x) ? 0.0f : a - back.x, isinf(back.y) ? 0.0f : b - back.y, T());
+#pragma unroll
+        for (int w = 0; w < CTAS; ++w) {
+            st_cluster_u32(u.hi + r * u.stride + c, w, hi);
+            st_cluster_u32(u.lo + r * u.stride + c, w, lo);
+        }
+    }
+    if (lane < CTAS) st_cluster_u32(u.factor + r, lane, __float_as_uint(down));
+}
+
+// The fragments of u's steps s and s + 1 of a lane's two rows (g and g + 8 from `u` on).
+template <int RANK16, typename T>
+__device__ __forceinline__ void u_fragments(const T* u, int stride, int s, int q, uint32_t (&f)[2][4]) {
+    if constexpr (RANK16 == 1) {
+        const uint2 a = *reinterpret_cast<const uint2*>(u + q * 4), b = *reinterpret_cast<const uint2*>(u + 8 * stride + q * 4);
+        f[0][0] = a.x, f[0][1] = b.x, f[0][2] = a.y, f[0][3] = b.y;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(u + s * 16 + q * 8);
+        const uint4 b = *reinterpret_cast<const uint4*>(u + 8 * stride + s * 16 + q * 8);
+        f[0][0] = a.x, f[0][1] = b.x, f[0][2] = a.y, f[0][3] = b.y;
+        f[1][0] = a.z, f[1][1] = b.z, f[1][2] = a.w, f[1][3] = b.w;
+    }
+}
+
+// u times a block of B into acc. The four n8 tiles of a block take columns so that a lane ends up with eight consecutive
+// ones: tile j's column c is 8 (c / 2) + 2 j + c % 2 of the block; w(j, s) gives the lane's values of B's row for its
+// column g of tile j (eight of steps s and s + 1; four of the one step of RANK16 1).
+template <typename T, int RANK16, typename W>
+__device__ __forceinline__ void second_product(float (&acc)[4][4], const T* hi_at, const T* lo_at, int stride, int r8, int q,
+                                               W w) {
+    uint32_t hi[2][4], lo[2][4];
+#pragma unroll
+    for (int s = 0; s < RANK16; s += 2) {
+        if (s * 16 >= r8) break;
+        uint4 k[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = w(j, s);
+        u_fragments<RANK16>(hi_at, stride, s, q, hi);
+        u_fragments<RANK16>(lo_at, stride, s, q, lo);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            mma<T>(acc[j], hi[0], k[j].x, k[j].y);
+            mma<T>(acc[j], lo[0], k[j].x, k[j].y);
+            if constexpr (RANK16 > 1) {
+                mma<T>(acc[j], hi[1], k[j].z, k[j].w);
+                mma<T>(acc[j], lo[1], k[j].z, k[j].w);
+            }
+        }
+    }
+}
+
+// Eight values of y plus f times a row of acc (e: 0 or 2, its first element), rounded once.
+template <typename T>
+__device__ __forceinline__ uint4 added(const uint4& y, const float (&acc)[4][4], int e, float f) {
+    uint4 o;
+    const uint32_t* from = &y.x;
+    uint32_t* to = &o.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 v = unpack(from[j], T());
+        to[j] = pack(fmaf(f, acc[j][e], v.x), fmaf(f, acc[j][e + 1], v.y), T());
+    }
+    return o;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows an adapter: tiles of 16 rows, eight CTAs of eight warps, operands straight from global memory, the loads of many
+// blocks of k asked for before the first product.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int FEW_ROWS = 16, FEW_WARPS = 8, FEW_CTAS = 8;
+
+template <typename T, int RANK16>
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2) adapt_few(AdaptParams p) {
+    constexpr int M = FEW_ROWS, WARPS = FEW_WARPS, THREADS = WARPS * 32, RP = RANK16 * 16;
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int tile_rows[M];
-    __shared__ int tile_slot, tile_count, found[2];
+    __shared__ int tile_slot, tile_count, found;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
-    const int rank = blockIdx.x % CTAS, tile = blockIdx.x / CTAS;
-    const int cap = p.ad.rank, K = p.ad.k, mats = p.ad.n_mats, cols = mats * RP, us = u_stride(cols);
-    float* sums = reinterpret_cast<float*>(smem);
-    T* u_hi = reinterpret_cast<T*>(sums + M * cols);
-    T* u_lo = u_hi + M * us;
-    float* factor = reinterpret_cast<float*>(u_lo + M * us);
+    const int rank = blockIdx.x % FEW_CTAS, tile = blockIdx.x / FEW_CTAS;
+    const Inner<T> u(smem, M, p.ad.n_mats * RP);
     pdl_launch_dependents();
     pdl_wait();
 
@@ -187,12 +351,12 @@ __global__ void __launch_bounds__(Shape<ROW_WARPS>::THREADS, 2) adapt_kernel(Ada
         const Tile mine = reinterpret_cast<const Tile*>(p.plan)[tile];
         if (mine.count == 0) return;        // (the whole cluster: one tile)
         const int* rows = p.plan + 4 * p.max_tiles + mine.first;
-        for (int i = tid; i < M; i += THREADS) tile_rows[i] = i < mine.count ? rows[i] : -1;
+        if (tid < M) tile_rows[tid] = tid < mine.count ? rows[tid] : -1;
         if (tid == 0) tile_slot = mine.slot, tile_count = mine.count;
     } else {
         // Tile j is row j's if the rows of its adapter before it fill whole tiles; it takes the next M of them.
         const int slot = slot_of(p, tile);
-        for (int i = tid; i < M; i += THREADS) tile_rows[i] = -1;
+        if (tid < M) tile_rows[tid] = -1;
         if (tid == 0) tile_slot = slot;
         __syncthreads();
         if (warp == 0) {
@@ -206,154 +370,246 @@ __global__ void __launch_bounds__(Shape<ROW_WARPS>::THREADS, 2) adapt_kernel(Ada
                 if ((same & from) >> lane & 1 && at < M) tile_rows[at] = t;
                 taken += __popc(same & from);
             }
-            if (lane == 0) tile_count = min(taken, M), found[0] = before % M == 0;
+            if (lane == 0) tile_count = min(taken, M), found = before % M == 0;
         }
         __syncthreads();
-        if (!found[0]) return;
+        if (!found) return;
     }
     __syncthreads();
     const int slot = tile_slot, count = tile_count;
-    int r8 = 0;             // the adapter's rank, in whole steps of 8
-    if (slot >= 0) r8 = p.ad.ranks ? (min(max(p.ad.ranks[slot], 0), cap) + 7) / 8 * 8 : cap;
+    const Adapter<T> ad(p, slot);
+    if (ad.r8 == 0) return copy_rows<T>(p, tile_rows, count, rank, FEW_CTAS, WARPS);
     const T* x = static_cast<const T*>(p.x);
     const T* y = static_cast<const T*>(p.y);
     T* out = static_cast<T*>(p.out);
-
-    // this CTA's 32-column blocks of the output, matrix by matrix
-    int blocks = 0;
-    for (int m = 0; m < mats; ++m) blocks += (p.ad.widths[m] + 31) / 32;
-    const int block_lo = blocks * rank / CTAS, block_hi = blocks * (rank + 1) / CTAS;
-
-    if (r8 == 0) {          // nothing to add: y itself
-        if (out == y && p.out_stride == p.y_stride) return;
-        const int from = p.n / 8 * rank / CTAS, to = p.n / 8 * (rank + 1) / CTAS;
-        for (int r = warp; r < count; r += WARPS)
-            for (int c = from + lane; c < to; c += 32)
-                reinterpret_cast<uint4*>(out + tile_rows[r] * p.out_stride)[c] =
-                    reinterpret_cast<const uint4*>(y + tile_rows[r] * p.y_stride)[c];
-        return;
+    const int blocks = block_count(p), block_lo = blocks * rank / FEW_CTAS, block_hi = blocks * (rank + 1) / FEW_CTAS;
+    if (block_lo < block_hi) {      // what the second product will read, into L2 meanwhile
+        const Block a = block_at(p, block_lo), z = block_at(p, block_hi - 1);
+        const int columns = z.col + min(z.left, 32) - a.col;
+        if (tid < count) prefetch_l2(y + tile_rows[tid] * p.y_stride + a.col, columns * sizeof(T));
+        if (tid == THREADS - 1)
+            prefetch_l2(ad.b + static_cast<size_t>(a.col) * ad.cap, static_cast<size_t>(columns) * ad.cap * sizeof(T));
     }
 
-    const T* B = static_cast<const T*>(p.ad.b) + static_cast<size_t>(slot) * p.n * cap;
-    {   // what the second product will read, into L2 meanwhile
-        int col_lo = p.n, col_hi = 0, first = 0, col = 0;
-        for (int m = 0; m < mats; ++m) {
-            const int w = p.ad.widths[m], n = (w + 31) / 32, from = max(block_lo - first, 0), to = min(block_hi - first, n);
-            if (from < to) col_lo = min(col_lo, col + from * 32), col_hi = max(col_hi, col + min(w, to * 32));
-            first += n, col += w;
-        }
-        if (col_lo < col_hi) {
-            if (tid < count) prefetch_l2(y + tile_rows[tid] * p.y_stride + col_lo, (col_hi - col_lo) * sizeof(T));
-            if (tid == THREADS - 1)
-                prefetch_l2(B + static_cast<size_t>(col_lo) * cap, static_cast<size_t>(col_hi - col_lo) * cap * sizeof(T));
-        }
-    }
-
-    // u = x A^T over this CTA's blocks of k. n8 tile t of the inner columns is ranks 8 j .. 8 j + 7 of matrix m, t = m
-    // (r8 / 8) + j.
-    const int k_blocks = (K + 31) / 32, k_lo = k_blocks * rank / CTAS, k_hi = k_blocks * (rank + 1) / CTAS;
-    const int tiles_a_mat = r8 / 8, n_tiles = mats * tiles_a_mat;
-    const T* A = static_cast<const T*>(p.ad.a) + static_cast<size_t>(slot) * mats * cap * K;
-    const int row_warp = ROW_WARPS == 1 ? 0 : warp % ROW_WARPS, col_warp = warp / ROW_WARPS;
-    const int ra = tile_rows[row_warp * 16 + g], rb = tile_rows[row_warp * 16 + g + 8];
+    const int ra = tile_rows[g], rb = tile_rows[g + 8], K = ad.k;
+    const int k_lo = segment_at((K + 31) / 32, rank), k_hi = segment_at((K + 31) / 32, rank + 1);
     const uint4 zero = {0, 0, 0, 0};
-    const auto a_row = [&](int t, int r) {      // row r of tile t of A
-        const int m = t / tiles_a_mat;
-        return A + (static_cast<size_t>(m) * cap + (t - m * tiles_a_mat) * 8 + r) * K;
-    };
-    const auto column = [&](int t) {            // its first column in sums and u
-        const int m = t / tiles_a_mat;
-        return m * RP + (t - m * tiles_a_mat) * 8;
-    };
-    if constexpr (ROW_WARPS == 1) {
-        const T* xa = ra >= 0 ? x + ra * p.x_stride : nullptr;
-        const T* xb = rb >= 0 ? x + rb * p.x_stride : nullptr;
-        // G tiles a warp at once (t0, t0 + WARPS, ...), U blocks of k asked for at once
-        const auto product = [&](auto G_, auto U_) {
-            constexpr int G = G_, U = U_;
-            for (int t0 = warp; t0 < n_tiles; t0 += G * WARPS) {
-                const T* from[G];
+    const T* xa = ra >= 0 ? x + ra * p.x_stride : nullptr;
+    const T* xb = rb >= 0 ? x + rb * p.x_stride : nullptr;
+    // G tiles a warp at once (t0, t0 + WARPS, ...), U blocks of k asked for at once
+    const auto first_product = [&](auto G_, auto U_) {
+        constexpr int G = G_, U = U_;
+        for (int t0 = warp; t0 < ad.n_tiles; t0 += G * WARPS) {
+            const T* from[G];
 #pragma unroll
-                for (int j = 0; j < G; ++j) from[j] = t0 + j * WARPS < n_tiles ? a_row(t0 + j * WARPS, g) : nullptr;
-                float acc[G][4] = {};
-                for (int k0 = k_lo; k0 < k_hi; k0 += U) {
-                    uint4 va[U], vb[U], w[U][G];
+            for (int j = 0; j < G; ++j) from[j] = t0 + j * WARPS < ad.n_tiles ? ad.a_row(t0 + j * WARPS, g) : nullptr;
+            float acc[G][4] = {};
+            for (int k0 = k_lo; k0 < k_hi; k0 += U) {
+                uint4 va[U], vb[U], w[U][G];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const int k = (k0 + u) * 32 + q * 8;
-                        const bool in = k0 + u < k_hi && k < K;
-                        va[u] = in && xa ? *reinterpret_cast<const uint4*>(xa + k) : zero;
-                        vb[u] = in && xb ? *reinterpret_cast<const uint4*>(xb + k) : zero;
+                for (int i = 0; i < U; ++i) {
+                    const int k = (k0 + i) * 32 + q * 8;
+                    const bool in = k0 + i < k_hi && k < K;
+                    va[i] = in && xa ? *reinterpret_cast<const uint4*>(xa + k) : zero;
+                    vb[i] = in && xb ? *reinterpret_cast<const uint4*>(xb + k) : zero;
 #pragma unroll
-                        for (int j = 0; j < G; ++j)
-                            w[u][j] = in && from[j] ? *reinterpret_cast<const uint4*>(from[j] + k) : zero;
-                    }
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const uint32_t a0[4] = {va[u].x, vb[u].x, va[u].y, vb[u].y};
-                        const uint32_t a1[4] = {va[u].z, vb[u].z, va[u].w, vb[u].w};
-                        if (k0 + u < k_hi)
-#pragma unroll
-                            for (int j = 0; j < G; ++j) {
-                                mma<T>(acc[j], a0, w[u][j].x, w[u][j].y);
-                                mma<T>(acc[j], a1, w[u][j].z, w[u][j].w);
-                            }
-                    }
+                    for (int j = 0; j < G; ++j)
+                        w[i][j] = in && from[j] ? *reinterpret_cast<const uint4*>(from[j] + k) : zero;
                 }
 #pragma unroll
-                for (int j = 0; j < G; ++j)
-                    if (from[j])
+                for (int i = 0; i < U; ++i) {
+                    const uint32_t a0[4] = {va[i].x, vb[i].x, va[i].y, vb[i].y};
+                    const uint32_t a1[4] = {va[i].z, vb[i].z, va[i].w, vb[i].w};
+                    if (k0 + i < k_hi)
 #pragma unroll
-                        for (int e = 0; e < 4; e += 2)
-                            *reinterpret_cast<float2*>(&sums[(g + e * 4) * cols + column(t0 + j * WARPS) + q * 2]) =
-                                make_float2(acc[j][e], acc[j][e + 1]);
-            }
-        };
-        if (n_tiles <= WARPS) product(std::integral_constant<int, 1>(), std::integral_constant<int, 6>());
-        else product(std::integral_constant<int, GROUP>(), std::integral_constant<int, 4>());
-    } else {
-        // A stage: M rows of x, then the rows of A, 128 bytes each; 16-byte piece c of row r lies at c ^ 4 (r % 2), so that
-        // the eight lanes of a quarter load (two rows, four pieces) meet every bank once.
-        const int a_rows = n_tiles * 8, n_stages = ((k_hi - k_lo) * 32 + STAGE_K - 1) / STAGE_K;
-        const auto fill = [&](int i) {
-            unsigned char* to = smem + (i % stages) * stage_bytes(cols);
-            const int k0 = k_lo * 32 + i * STAGE_K;
-            for (int piece = tid; piece < (M + a_rows) * 8; piece += THREADS) {
-                const int r = piece >> 3, c = piece & 7, k = k0 + c * 8;
-                const T* from = nullptr;
-                if (k < k_hi * 32 && k < K) {
-                    if (r >= M) from = a_row((r - M) >> 3, (r - M) & 7) + k;
-                    else if (tile_rows[r] >= 0) from = x + tile_rows[r] * p.x_stride + k;
+                        for (int j = 0; j < G; ++j) {
+                            mma<T>(acc[j], a0, w[i][j].x, w[i][j].y);
+                            mma<T>(acc[j], a1, w[i][j].z, w[i][j].w);
+                        }
                 }
-                uint4* at = reinterpret_cast<uint4*>(to + r * 128 + (c ^ (r & 1) << 2) * 16);
-                if (from) cp_async16(at, from);
-                else *at = zero;
             }
-        };
-        const int per = (n_tiles + COL_WARPS - 1) / COL_WARPS, t0 = col_warp * per, nt = min(per, n_tiles - t0);
-        float acc[GROUP][4] = {};
-        for (int i = 0; i < stages - 1; ++i) {
-            if (i < n_stages) fill(i);
-            cp_async_commit();
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+                if (from[j])
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2)
+                        *reinterpret_cast<float2*>(
+                            &u.sums[(g + e * 4) * u.cols + ad.template column<RP>(t0 + j * WARPS) + q * 2]) =
+                            make_float2(acc[j][e], acc[j][e + 1]);
         }
-        for (int i = 0; i < n_stages; ++i) {
-            if (stages == 4) cp_async_wait<2>();        // the stage after this and the one behind it may be on their way
-            else cp_async_wait<1>();
-            __syncthreads();
-            if (i + stages - 1 < n_stages) fill(i + stages - 1);
-            cp_async_commit();
-            const unsigned char* from = smem + (i % stages) * stage_bytes(cols);
+    };
+    if (ad.n_tiles <= WARPS) first_product(std::integral_constant<int, 1>(), std::integral_constant<int, 6>());
+    else first_product(std::integral_constant<int, 3>(), std::integral_constant<int, 4>());
+    cluster_sync_all();
+    const float scale = p.ad.scales ? p.ad.scales[slot] : 1.0f;
+    for (int r = rank * (M / FEW_CTAS) + warp; r < (rank + 1) * (M / FEW_CTAS); r += WARPS)
+        join_row<T, RANK16, FEW_CTAS>(u, r, ad.r8, scale);
+    cluster_sync_all();     // (the last access to another CTA's memory was before it)
+
+    const float fa = u.factor[g], fb = u.factor[g + 8];
+    for (int b = block_lo + warp; b < block_hi; b += WARPS) {
+        const Block block = block_at(p, b);
+        const int col = block.col + q * 8;
+        const bool in = q * 8 < block.left, n_in = (g >> 1) * 8 < block.left;
+        const uint4 ya = in && ra >= 0 ? *reinterpret_cast<const uint4*>(y + ra * p.y_stride + col) : zero;
+        const uint4 yb = in && rb >= 0 ? *reinterpret_cast<const uint4*>(y + rb * p.y_stride + col) : zero;
+        const T* w = ad.b + (static_cast<size_t>(block.col) + (g >> 1) * 8 + (g & 1)) * ad.cap;
+        float acc[4][4] = {};
+        const size_t at = g * u.stride + block.m * RP;
+        second_product<T, RANK16>(acc, u.hi + at, u.lo + at, u.stride, ad.r8, q, [&](int j, int s) {
+            if constexpr (RANK16 == 1) {
+                const uint2 v = n_in && q * 4 < ad.r8 ? *reinterpret_cast<const uint2*>(w + j * 2 * ad.cap + q * 4) : uint2{0, 0};
+                return uint4{v.x, v.y, 0, 0};
+            } else {
+                return n_in && s * 16 + q * 8 < ad.r8 ? *reinterpret_cast<const uint4*>(w + j * 2 * ad.cap + s * 16 + q * 8)
+                                                      : zero;
+            }
+        });
+        if (in && ra >= 0) *reinterpret_cast<uint4*>(out + ra * p.out_stride + col) = added<T>(ya, acc, 0, fa);
+        if (in && rb >= 0) *reinterpret_cast<uint4*>(out + rb * p.out_stride + col) = added<T>(yb, acc, 2, fb);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Many rows an adapter (prefill): tiles of 64 rows, sixteen warps (four row groups by four shares of the columns), CTAS a
+// cluster. One ring of shared memory carries both products: stages of 64 k of x and A, then stages of 128 columns of y and
+// B, filled by 16-byte asynchronous copies, so that the second product's operands are on their way while the sums are
+// joined. Rows of a stage are 128 bytes or more apart and their 16-byte pieces swapped by halves on odd rows (piece ^ 4),
+// so that a quarter load (two rows, four pieces) meets every bank once.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int MANY_ROWS = 64, MANY_WARPS = 16, MANY_TILES = 6, MANY_COLS = MANY_TILES * 8 * 4;      // inner columns it holds
+constexpr int stage_bytes(int cols, int rank16) {
+    const int first = (MANY_ROWS + cols) * 128, second = MANY_ROWS * 256 + 128 * rank16 * 32;
+    return first > second ? first : second;
+}
+constexpr int many_bytes(int cols, int rank16, int stages, int ctas) {
+    const int levels = (ctas >= 4 ? 1 : 2) * sums_bytes(MANY_ROWS, cols), halves = halves_bytes(MANY_ROWS, cols);
+    return stages * stage_bytes(cols, rank16) + sums_bytes(MANY_ROWS, cols) + (ctas < 8 && levels > halves ? levels : halves);
+}
+
+template <typename T, int RANK16, int CTAS>
+__global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_many(AdaptParams p, int stages) {
+    constexpr int M = MANY_ROWS, WARPS = MANY_WARPS, THREADS = WARPS * 32, RP = RANK16 * 16, OWN = SEGMENTS / CTAS;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int tile_rows[M];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    const int row_warp = warp & 3, col_warp = warp >> 2;
+    const int rank = blockIdx.x % CTAS, tile = blockIdx.x / CTAS;
+    const int cols = p.ad.n_mats * RP, slot_bytes = stage_bytes(cols, RANK16);
+    const Inner<T> u(smem + stages * slot_bytes, M, cols);
+    pdl_launch_dependents();
+    pdl_wait();
+    const Tile mine = reinterpret_cast<const Tile*>(p.plan)[tile];
+    if (mine.count == 0) return;        // (the whole cluster: one tile)
+    if (tid < M) tile_rows[tid] = tid < mine.count ? p.plan[4 * p.max_tiles + mine.first + tid] : -1;
+    __syncthreads();
+    const Adapter<T> ad(p, mine.slot);
+    if (ad.r8 == 0) return copy_rows<T>(p, tile_rows, mine.count, rank, CTAS, WARPS);
+    const T* x = static_cast<const T*>(p.x);
+    const T* y = static_cast<const T*>(p.y);
+    T* out = static_cast<T*>(p.out);
+    const int K = ad.k, k_blocks = (K + 31) / 32, a_rows = ad.n_tiles * 8;
+    const int blocks = block_count(p), block_lo = blocks * rank / CTAS, block_hi = blocks * (rank + 1) / CTAS;
+    const uint4 zero = {0, 0, 0, 0};
+
+    // Stages of the first product: each segment of k by itself, two blocks of 32 a stage.
+    int n_first = 0;
 #pragma unroll
-            for (int h = 0; h < STAGE_K / 32; ++h) {
-                const int kb = k_lo + i * (STAGE_K / 32) + h;
-                if (kb >= k_hi) break;
+    for (int s = 0; s < OWN; ++s)
+        n_first += (segment_at(k_blocks, rank * OWN + s + 1) - segment_at(k_blocks, rank * OWN + s) + 1) / 2;
+    const int n_second = (block_hi - block_lo + 3) / 4, n_stages = n_first + n_second;
+    const auto put = [&](unsigned char* to, const T* from) {
+        if (from) cp_async16(to, from);
+        else *reinterpret_cast<uint4*>(to) = zero;
+    };
+    // This thread's pieces of a first stage: rows of x, then of A.
+    constexpr int PIECES = (MANY_ROWS + MANY_COLS) * 8 / THREADS;
+    const T* piece_from[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int r = (tid + i * THREADS) >> 3, c = tid & 7;
+        piece_from[i] = nullptr;
+        if (r < M) piece_from[i] = tile_rows[r] >= 0 ? x + tile_rows[r] * p.x_stride + c * 8 : nullptr;
+        else if (r < M + a_rows) piece_from[i] = ad.a_row((r - M) >> 3, (r - M) & 7) + c * 8;
+    }
+    int fill_stage = 0, fill_segment = rank * OWN, fill_block = segment_at(k_blocks, rank * OWN);
+    const auto fill = [&] {         // the next stage
+        if (fill_stage >= n_stages) return;
+        unsigned char* to = smem + fill_stage % stages * slot_bytes;
+        if (fill_stage < n_first) {
+            while (fill_block >= segment_at(k_blocks, fill_segment + 1)) ++fill_segment;
+            const int k = fill_block * 32 + (tid & 7) * 8, end = min(segment_at(k_blocks, fill_segment + 1) * 32, K);
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int r = (tid + i * THREADS) >> 3, c = tid & 7;
+                if (r < M + a_rows)
+                    put(to + r * 128 + (c ^ (r & 1) << 2) * 16, k < end && piece_from[i] ? piece_from[i] + fill_block * 32 : nullptr);
+            }
+            fill_block = min(fill_block + 2, segment_at(k_blocks, fill_segment + 1));
+        } else {
+            const int b0 = block_lo + (fill_stage - n_first) * 4;
+            // y: [row][16 pieces], four blocks of four
+#pragma unroll
+            for (int i = 0; i < M * 16 / THREADS; ++i) {
+                const int r = (tid + i * THREADS) >> 4, c = tid & 15, b = b0 + (c >> 2);
+                const T* from = nullptr;
+                if (tile_rows[r] >= 0 && b < block_hi) {
+                    const Block block = block_at(p, b);
+                    if ((c & 3) * 8 < block.left) from = y + tile_rows[r] * p.y_stride + block.col + (c & 3) * 8;
+                }
+                put(to + r * 256 + (c ^ (r & 1) << 2) * 16, from);
+            }
+            // B: [block][j][g][RP]: row g of tile j is the block's column 8 (g / 2) + 2 j + g % 2
+            constexpr int ROW = RANK16 * 2;     // pieces of a row
+#pragma unroll
+            for (int i = tid; i < 128 * ROW; i += THREADS) {
+                const int row = i / ROW, c = i % ROW, b = b0 + (row >> 5), j = row >> 3 & 3, gg = row & 7;
+                const int n = (gg >> 1) * 8 + j * 2 + (gg & 1);
+                const T* from = nullptr;
+                if (b < block_hi && c * 8 < ad.r8) {
+                    const Block block = block_at(p, b);
+                    if (n < block.left) from = ad.b + (static_cast<size_t>(block.col) + n) * ad.cap + c * 8;
+                }
+                put(to + M * 256 + row * ROW * 16 + (ROW >= 8 ? c ^ (row & 1) << 2 : c) * 16, from);
+            }
+        }
+        ++fill_stage;
+    };
+    for (int i = 0; i < stages - 1; ++i) fill(), cp_async_commit();
+    int stage = 0;
+    const auto next = [&] {         // the next stage, whole and for all; the one behind it is filled again
+        if (stages == 4) cp_async_wait<2>();
+        else cp_async_wait<1>();
+        __syncthreads();
+        fill();
+        cp_async_commit();
+        return smem + stage++ % stages * slot_bytes;
+    };
+
+    // u = x A^T, a segment at a time; sums of segments join as the tree's levels complete (level l of this thread's values
+    // in shared memory, where u's halves will be).
+    const int per = (ad.n_tiles + 3) / 4, t0 = col_warp * per, nt = min(per, ad.n_tiles - t0);
+    float* levels = reinterpret_cast<float*>(u.hi);
+    const auto place = [&](float* base, int j, int e) {
+        return reinterpret_cast<float2*>(
+            &base[(row_warp * 16 + g + e * 4) * cols + ad.template column<RP>(t0 + j) + q * 2]);
+    };
+#pragma unroll
+    for (int s = 0; s < OWN; ++s) {
+        float acc[MANY_TILES][4] = {};
+        const int end = segment_at(k_blocks, rank * OWN + s + 1);
+        for (int kb = segment_at(k_blocks, rank * OWN + s); kb < end; kb += 2) {
+            const unsigned char* from = next();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (kb + h >= end) break;
                 const auto piece = [&](int r) {
                     return *reinterpret_cast<const uint4*>(from + r * 128 + ((h * 4 + q) ^ (r & 1) << 2) * 16);
                 };
                 const uint4 va = piece(row_warp * 16 + g), vb = piece(row_warp * 16 + g + 8);
                 const uint32_t a0[4] = {va.x, vb.x, va.y, vb.y}, a1[4] = {va.z, vb.z, va.w, vb.w};
 #pragma unroll
-                for (int j = 0; j < GROUP; ++j)
+                for (int j = 0; j < MANY_TILES; ++j)
                     if (j < nt) {
                         const uint4 w = piece(M + (t0 + j) * 8 + g);
                         mma<T>(acc[j], a0, w.x, w.y);
@@ -361,164 +617,81 @@ __global__ void __launch_bounds__(Shape<ROW_WARPS>::THREADS, 2) adapt_kernel(Ada
                     }
             }
         }
-        cp_async_wait<0>();
-        __syncthreads();        // the ring's place is free for the sums
 #pragma unroll
-        for (int j = 0; j < GROUP; ++j)
+        for (int j = 0; j < MANY_TILES; ++j)
             if (j < nt)
 #pragma unroll
-                for (int e = 0; e < 4; e += 2)
-                    *reinterpret_cast<float2*>(&sums[(row_warp * 16 + g + e * 4) * cols + column(t0 + j) + q * 2]) =
-                        make_float2(acc[j][e], acc[j][e + 1]);
+                for (int e = 0; e < 4; e += 2) {
+                    float2 v = make_float2(acc[j][e], acc[j][e + 1]);
+                    int level = 0;
+#pragma unroll
+                    for (int odd = s; odd & 1; odd >>= 1, ++level) {
+                        const float2 o = *place(levels + level * M * cols, j, e);
+                        v.x = o.x + v.x, v.y = o.y + v.y;
+                    }
+                    *place(s == OWN - 1 ? u.sums : levels + level * M * cols, j, e) = v;
+                }
     }
     cluster_sync_all();
-
-    // Add up the eight CTAs' sums of this CTA's eighth of the rows, in rank order, and store them into all eight as two
-    // 16-bit halves (hi + lo is the sum to 2^-16 of it, so the second product rounds nothing that the output shows). For
-    // fp16 a row is first scaled by a power of two that brings its largest value to [2^14, 2^15); the factor comes back
-    // with the adapter's scale.
-    const float scale = p.ad.scales ? p.ad.scales[slot] : 1.0f;
-    for (int r = rank * (M / CTAS) + warp; r < (rank + 1) * (M / CTAS); r += WARPS) {
-        float2 v[RANK16];
-        float top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < RANK16; ++i) {
-            const int c = lane * 2 + i * 64;
-            v[i] = {0.0f, 0.0f};
-            if (c < cols && c % RP < r8)
-#pragma unroll
-                for (int w = 0; w < CTAS; ++w) {
-                    const float2 o = ld_cluster_f2(sums + r * cols + c, w);
-                    v[i].x += o.x, v[i].y += o.y;
-                }
-            top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
-        }
-        float up = 1.0f, down = scale;
-        if constexpr (std::is_same_v<T, __half>) {
-            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-            if (top > 1e-30f && top < 1e30f) {
-                const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
-                up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                down = scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < RANK16; ++i) {
-            const int c = lane * 2 + i * 64;
-            if (c >= cols) continue;
-            const float a = v[i].x * up, b = v[i].y * up;
-            const uint32_t hi = pack(a, b, T());
-            const float2 back = unpack(hi, T());
-            // (an infinite half leaves nothing to the other one)
-            const uint32_t lo = pack(isinf(back.x) ? 0.0f : a - back.x, isinf(back.y) ? 0.0f : b - back.y, T());
-#pragma unroll
-            for (int w = 0; w < CTAS; ++w) {
-                st_cluster_u32(u_hi + r * us + c, w, hi);
-                st_cluster_u32(u_lo + r * us + c, w, lo);
-            }
-        }
-        if (lane < CTAS) st_cluster_u32(factor + r, lane, __float_as_uint(down));
-    }
+    const float scale = p.ad.scales ? p.ad.scales[mine.slot] : 1.0f;
+    for (int r = rank * (M / CTAS) + warp; r < (rank + 1) * (M / CTAS); r += WARPS)
+        join_row<T, RANK16, CTAS>(u, r, ad.r8, scale);
     cluster_sync_all();     // (the last access to another CTA's memory was before it)
 
-    // out = y + factor u B^T over this CTA's blocks of columns. The four n8 tiles of a block take columns so that a lane ends
-    // up with eight consecutive ones: tile j's column c is 8 (c / 2) + 2 j + c % 2 of the block.
-    const float fa = factor[row_warp * 16 + g], fb = factor[row_warp * 16 + g + 8];
-    int m = -1, m_block = 0, m_col = 0, next_block = 0;       // the matrix of the block, its first block and column
-    const T *h_at = nullptr, *l_at = nullptr;                 // this lane's halves of u for that matrix
-    const auto halves = [&](const T* u, int s, uint32_t (&f)[2][4]) {       // the fragments of steps s and s + 1
-        if constexpr (RANK16 == 1) {
-            const uint2 va = *reinterpret_cast<const uint2*>(u + q * 4), vb = *reinterpret_cast<const uint2*>(u + 8 * us + q * 4);
-            f[0][0] = va.x, f[0][1] = vb.x, f[0][2] = va.y, f[0][3] = vb.y;
-        } else {
-            const uint4 va = *reinterpret_cast<const uint4*>(u + s * 16 + q * 8);
-            const uint4 vb = *reinterpret_cast<const uint4*>(u + 8 * us + s * 16 + q * 8);
-            f[0][0] = va.x, f[0][1] = vb.x, f[0][2] = va.y, f[0][3] = vb.y;
-            f[1][0] = va.z, f[1][1] = vb.z, f[1][2] = va.w, f[1][3] = vb.w;
-        }
-    };
-    for (int b = block_lo + col_warp; b < block_hi; b += COL_WARPS) {
-        if (b >= next_block) {
-            while (b >= next_block) {
-                if (m >= 0) m_col += p.ad.widths[m];
-                m_block = next_block;
-                next_block += (p.ad.widths[++m] + 31) / 32;
-            }
-            h_at = u_hi + (row_warp * 16 + g) * us + m * RP;
-            l_at = u_lo + (row_warp * 16 + g) * us + m * RP;
-        }
-        const int width = p.ad.widths[m], base = (b - m_block) * 32;      // columns of matrix m
-        const bool in = base + q * 8 < width;
-        const int col = m_col + base + q * 8;
-        const uint4 ya = in && ra >= 0 ? *reinterpret_cast<const uint4*>(y + ra * p.y_stride + col) : zero;
-        const uint4 yb = in && rb >= 0 ? *reinterpret_cast<const uint4*>(y + rb * p.y_stride + col) : zero;
-        const bool n_in = base + (g >> 1) * 8 < width;
-        const T* w = B + (static_cast<size_t>(m_col) + base + (g >> 1) * 8 + (g & 1)) * cap;
-        float acc[4][4] = {};
-        uint32_t hi[2][4], lo[2][4];
-        if constexpr (RANK16 == 1) {
-            uint2 k[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                k[j] = n_in && q * 4 < r8 ? *reinterpret_cast<const uint2*>(w + j * 2 * cap + q * 4) : uint2{0, 0};
-            halves(h_at, 0, hi);
-            halves(l_at, 0, lo);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                mma<T>(acc[j], hi[0], k[j].x, k[j].y);
-                mma<T>(acc[j], lo[0], k[j].x, k[j].y);
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < RANK16; s += 2) {
-                if (s * 16 >= r8) break;
-                uint4 k[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    k[j] = n_in && s * 16 + q * 8 < r8 ? *reinterpret_cast<const uint4*>(w + j * 2 * cap + s * 16 + q * 8)
-                                                       : zero;
-                halves(h_at, s, hi);
-                halves(l_at, s, lo);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    mma<T>(acc[j], hi[0], k[j].x, k[j].y);
-                    mma<T>(acc[j], lo[0], k[j].x, k[j].y);
-                    mma<T>(acc[j], hi[1], k[j].z, k[j].w);
-                    mma<T>(acc[j], lo[1], k[j].z, k[j].w);
-                }
-            }
-        }
-        if (!in) continue;
-        const auto add = [&](const uint4& v, int e, float f) {
-            uint4 o;
-            const uint32_t* from = &v.x;
-            uint32_t* to = &o.x;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 b2 = unpack(from[j], T());
-                to[j] = pack(fmaf(f, acc[j][e], b2.x), fmaf(f, acc[j][e + 1], b2.y), T());
-            }
-            return o;
+    const int la = row_warp * 16 + g, lb = la + 8, ra = tile_rows[la], rb = tile_rows[lb];
+    const float fa = u.factor[la], fb = u.factor[lb];
+    for (int i = 0; i < n_second; ++i) {
+        const unsigned char* from = next();
+        const int b = block_lo + i * 4 + col_warp;
+        if (b >= block_hi) continue;
+        const Block block = block_at(p, b);
+        const auto y_piece = [&](int r) {
+            return *reinterpret_cast<const uint4*>(from + r * 256 + ((col_warp * 4 + q) ^ (r & 1) << 2) * 16);
         };
-        if (ra >= 0) *reinterpret_cast<uint4*>(out + ra * p.out_stride + col) = add(ya, 0, fa);
-        if (rb >= 0) *reinterpret_cast<uint4*>(out + rb * p.out_stride + col) = add(yb, 2, fb);
+        const unsigned char* w = from + M * 256 + (col_warp * 32 + g) * RANK16 * 32;
+        float acc[4][4] = {};
+        const size_t at = la * u.stride + block.m * RP;
+        second_product<T, RANK16>(acc, u.hi + at, u.lo + at, u.stride, ad.r8, q, [&](int j, int s) {
+            const unsigned char* row = w + j * 8 * RANK16 * 32;
+            if constexpr (RANK16 == 1) {
+                const uint2 v = *reinterpret_cast<const uint2*>(row + q * 8);
+                return uint4{v.x, v.y, 0, 0};
+            } else {
+                const int c = s * 2 + q;
+                return *reinterpret_cast<const uint4*>(row + (RANK16 >= 4 ? c ^ (g & 1) << 2 : c) * 16);
+            }
+        });
+        if (q * 8 >= block.left) continue;
+        const int col = block.col + q * 8;
+        if (ra >= 0) *reinterpret_cast<uint4*>(out + ra * p.out_stride + col) = added<T>(y_piece(la), acc, 0, fa);
+        if (rb >= 0) *reinterpret_cast<uint4*>(out + rb * p.out_stride + col) = added<T>(y_piece(lb), acc, 2, fb);
     }
+    cp_async_wait<0>();
 }
 
-using Kernel = void (*)(AdaptParams, int);
-
-template <typename T, int ROW_WARPS>
-Kernel kernel_of(int rank16) {
-    return rank16 == 1   ? adapt_kernel<T, ROW_WARPS, 1>
-           : rank16 == 2 ? adapt_kernel<T, ROW_WARPS, 2>
-           : rank16 == 4 ? adapt_kernel<T, ROW_WARPS, 4>
-                         : adapt_kernel<T, ROW_WARPS, 8>;
+template <typename T>
+auto few_kernel(int rank16) -> void (*)(AdaptParams) {
+    return rank16 == 1 ? adapt_few<T, 1> : rank16 == 2 ? adapt_few<T, 2> : rank16 == 4 ? adapt_few<T, 4> : adapt_few<T, 8>;
+}
+template <typename T, int CTAS>
+auto many_kernel(int rank16) -> void (*)(AdaptParams, int) {
+    return rank16 == 1   ? adapt_many<T, 1, CTAS>
+           : rank16 == 2 ? adapt_many<T, 2, CTAS>
+           : rank16 == 4 ? adapt_many<T, 4, CTAS>
+                         : adapt_many<T, 8, CTAS>;
+}
+template <typename T>
+auto many_kernel(int rank16, int ctas) {
+    return ctas == 2 ? many_kernel<T, 2>(rank16) : ctas == 4 ? many_kernel<T, 4>(rank16) : many_kernel<T, 8>(rank16);
 }
 
 int rank_steps(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 
 // Tiles a plan may need: every adapter's rows (and those without one) end with a tile that is not full.
 long long max_tiles(int rows, int slots, int m) { return (rows + m - 1) / m + (rows < slots + 1 ? rows : slots + 1); }
+
+constexpr int MAX_SMEM = 226 * 1024;    // a CTA's dynamic shared memory, beside its few static words
+constexpr double CTA_COST = 0.06;       // of a tile's work, what a CTA spends on joining sums whatever its share is
 
 }  // namespace
 }  // namespace esp
@@ -559,14 +732,9 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
 
     const int steps = rank_steps(ad->rank), cols = ad->n_mats * steps * 16;
     const bool half = ad->dtype == F16;
-    // Tiles of 64 rows where adapters have that many on average and their shared memory lets two CTAs on an SM.
-    const bool wide = t_rows > NO_PLAN && t_rows / ad->slots >= 32 && cols <= WIDE_COLS;
-    const int m = wide ? Shape<4>::M : Shape<1>::M, threads = wide ? Shape<4>::THREADS : Shape<1>::THREADS;
-    const int stages = MAX_STAGES * stage_bytes(cols) <= 100 * 1024 ? MAX_STAGES : 3;
-    const size_t smem = wide ? std::max(joined_bytes<4>(cols), stages * stage_bytes(cols))
-                             : joined_bytes<1>(cols);
-    const Kernel kernel = wide ? (half ? kernel_of<__half, 4>(steps) : kernel_of<__nv_bfloat16, 4>(steps))
-                               : (half ? kernel_of<__half, 1>(steps) : kernel_of<__nv_bfloat16, 1>(steps));
+    // Tiles of 64 rows where adapters have half of that on average and their inner columns fit a CTA.
+    const bool many = t_rows > NO_PLAN && t_rows / ad->slots >= 32 && cols <= MANY_COLS;
+    const int m = many ? MANY_ROWS : FEW_ROWS;
     AdaptParams p{*ad, x, y, ids, out, nullptr, x_stride, y_stride, out_stride, t_rows, static_cast<int>(n), t_rows};
     if (t_rows > NO_PLAN) {
         p.max_tiles = static_cast<int>(max_tiles(t_rows, ad->slots, m));
@@ -576,9 +744,31 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
                                   reinterpret_cast<int*>(tiles + p.max_tiles), m))
             return rc;
     }
-    if (const int rc = allow_smem(kernel, smem)) return rc;
-    if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * CTAS), dim3(threads), smem, stream,
-                                      true, CTAS, p, stages))
+    if (!many) {
+        const auto kernel = half ? few_kernel<__half>(steps) : few_kernel<__nv_bfloat16>(steps);
+        const size_t smem = sums_bytes(m, cols) + halves_bytes(m, cols);
+        if (const int rc = allow_smem(kernel, std::max<size_t>(smem, 49153))) return rc;
+        if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * FEW_CTAS), dim3(FEW_WARPS * 32),
+                                          smem, stream, true, FEW_CTAS, p))
+            return rc;
+        return ok();
+    }
+    // CTAs a tile: as few as fill the GPU's places (two CTAs an SM, one from rank 33 on) in the fewest rounds of work.
+    const int places = device_sms() * (steps >= 4 ? 1 : 2), tiles = (t_rows + m - 1) / m + std::min(ad->slots, t_rows / m) / 2;
+    int ctas = 8;
+    double best = 1e30;
+    for (int c : {2, 4, 8}) {
+        if (many_bytes(cols, steps, 3, c) > MAX_SMEM) continue;
+        const double work = ((tiles * c + places - 1) / places) * (1.0 / c + CTA_COST);
+        if (work < best) best = work, ctas = c;
+    }
+    const int room = steps >= 4 ? MAX_SMEM : MAX_SMEM / 2 - 1024;
+    const int stages = many_bytes(cols, steps, 4, ctas) <= room ? 4 : 3;
+    const size_t smem = many_bytes(cols, steps, stages, ctas);
+    const auto kernel = half ? many_kernel<__half>(steps, ctas) : many_kernel<__nv_bfloat16>(steps, ctas);
+    if (const int rc = allow_smem(kernel, std::max<size_t>(smem, 49153))) return rc;
+    if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * ctas), dim3(MANY_WARPS * 32), smem,
+                                      stream, true, ctas, p, stages))
         return rc;
     return ok();
 }
