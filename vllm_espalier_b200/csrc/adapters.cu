@@ -518,72 +518,83 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
     for (int s = 0; s < OWN; ++s)
         n_first += (segment_at(k_blocks, rank * OWN + s + 1) - segment_at(k_blocks, rank * OWN + s) + 1) / 2;
     const int n_second = (block_hi - block_lo + 3) / 4, n_stages = n_first + n_second;
-    const auto put = [&](unsigned char* to, const T* from) {
-        if (from) cp_async16(to, from);
-        else *reinterpret_cast<uint4*>(to) = zero;
-    };
-    // This thread's pieces of a first stage: rows of x, then of A.
-    constexpr int PIECES = (MANY_ROWS + MANY_COLS) * 8 / THREADS;
-    const T* piece_from[PIECES];
+    // What this thread copies of a first stage: piece tid % 8 of rows tid / 8 + 64 i of x (i = 0), then of A; of a second:
+    // piece tid % 16 of rows tid / 16 + 32 i of y, then of B's. Rows of x and y that the tile lacks are left as they are (no
+    // other row's result has anything of theirs).
+    constexpr int PIECES = (MANY_ROWS + MANY_COLS) * 8 / THREADS, ROW = RANK16 * 2;     // ROW: pieces of a row of B
+    static_assert(MANY_ROWS * 8 == THREADS, "a piece of x a thread");
+    const int piece = tid & 7, piece_row = tid >> 3;
+    const T* from_first[PIECES];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-        const int r = (tid + i * THREADS) >> 3, c = tid & 7;
-        piece_from[i] = nullptr;
-        if (r < M) piece_from[i] = tile_rows[r] >= 0 ? x + tile_rows[r] * p.x_stride + c * 8 : nullptr;
-        else if (r < M + a_rows) piece_from[i] = ad.a_row((r - M) >> 3, (r - M) & 7) + c * 8;
+        const int a = piece_row + (i - 1) * MANY_ROWS;
+        if (i == 0) from_first[i] = tile_rows[piece_row] >= 0 ? x + tile_rows[piece_row] * p.x_stride + piece * 8 : nullptr;
+        else from_first[i] = a < a_rows ? ad.a_row(a >> 3, a & 7) + piece * 8 : nullptr;
     }
-    int fill_stage = 0, fill_segment = rank * OWN, fill_block = segment_at(k_blocks, rank * OWN);
+    const T* from_y[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = tile_rows[(tid >> 4) + i * 32];
+        from_y[i] = t >= 0 ? y + t * p.y_stride + (tid & 3) * 8 : nullptr;
+    }
+    const uint32_t to_first = piece_row * 128 + (piece ^ (piece_row & 1) << 2) * 16;
+    const uint32_t to_y = (tid >> 4) * 256 + ((tid & 15) ^ (tid >> 4 & 1) << 2) * 16;
+    int fill_stage = 0, fill_slot = 0, fill_segment = rank * OWN, fill_block = segment_at(k_blocks, fill_segment);
+    int fill_end = segment_at(k_blocks, fill_segment + 1);
     const auto fill = [&] {         // the next stage
         if (fill_stage >= n_stages) return;
-        unsigned char* to = smem + fill_stage % stages * slot_bytes;
+        unsigned char* to = smem + fill_slot * slot_bytes;
         if (fill_stage < n_first) {
-            while (fill_block >= segment_at(k_blocks, fill_segment + 1)) ++fill_segment;
-            const int k = fill_block * 32 + (tid & 7) * 8, end = min(segment_at(k_blocks, fill_segment + 1) * 32, K);
+            while (fill_block >= fill_end) fill_end = segment_at(k_blocks, ++fill_segment + 1);
+            const int k = fill_block * 32;
+            if (k + piece * 8 < min(fill_end * 32, K)) {
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                const int r = (tid + i * THREADS) >> 3, c = tid & 7;
-                if (r < M + a_rows)
-                    put(to + r * 128 + (c ^ (r & 1) << 2) * 16, k < end && piece_from[i] ? piece_from[i] + fill_block * 32 : nullptr);
+                for (int i = 0; i < PIECES; ++i)
+                    if (from_first[i]) cp_async16(to + to_first + i * MANY_ROWS * 128, from_first[i] + k);
+            } else {
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i)
+                    if (i == 0 || from_first[i]) *reinterpret_cast<uint4*>(to + to_first + i * MANY_ROWS * 128) = zero;
             }
-            fill_block = min(fill_block + 2, segment_at(k_blocks, fill_segment + 1));
+            fill_block = min(fill_block + 2, fill_end);
         } else {
-            const int b0 = block_lo + (fill_stage - n_first) * 4;
             // y: [row][16 pieces], four blocks of four
+            const int b0 = block_lo + (fill_stage - n_first) * 4, by = b0 + (tid >> 2 & 3);
+            if (by < block_hi) {
+                const Block block = block_at(p, by);
+                if ((tid & 3) * 8 < block.left)
 #pragma unroll
-            for (int i = 0; i < M * 16 / THREADS; ++i) {
-                const int r = (tid + i * THREADS) >> 4, c = tid & 15, b = b0 + (c >> 2);
-                const T* from = nullptr;
-                if (tile_rows[r] >= 0 && b < block_hi) {
-                    const Block block = block_at(p, b);
-                    if ((c & 3) * 8 < block.left) from = y + tile_rows[r] * p.y_stride + block.col + (c & 3) * 8;
-                }
-                put(to + r * 256 + (c ^ (r & 1) << 2) * 16, from);
+                    for (int i = 0; i < 2; ++i)
+                        if (from_y[i]) cp_async16(to + to_y + i * 32 * 256, from_y[i] + block.col);
             }
             // B: [block][j][g][RP]: row g of tile j is the block's column 8 (g / 2) + 2 j + g % 2
-            constexpr int ROW = RANK16 * 2;     // pieces of a row
 #pragma unroll
             for (int i = tid; i < 128 * ROW; i += THREADS) {
                 const int row = i / ROW, c = i % ROW, b = b0 + (row >> 5), j = row >> 3 & 3, gg = row & 7;
                 const int n = (gg >> 1) * 8 + j * 2 + (gg & 1);
-                const T* from = nullptr;
-                if (b < block_hi && c * 8 < ad.r8) {
-                    const Block block = block_at(p, b);
-                    if (n < block.left) from = ad.b + (static_cast<size_t>(block.col) + n) * ad.cap + c * 8;
-                }
-                put(to + M * 256 + row * ROW * 16 + (ROW >= 8 ? c ^ (row & 1) << 2 : c) * 16, from);
+                unsigned char* at = to + M * 256 + row * ROW * 16 + (ROW >= 8 ? c ^ (row & 1) << 2 : c) * 16;
+                if (b >= block_hi) continue;
+                const Block block = block_at(p, b);
+                if (n < block.left && c * 8 < ad.r8)
+                    cp_async16(at, ad.b + (static_cast<size_t>(block.col) + n) * ad.cap + c * 8);
+                else
+                    *reinterpret_cast<uint4*>(at) = zero;
             }
         }
         ++fill_stage;
+        if (++fill_slot == stages) fill_slot = 0;
     };
     for (int i = 0; i < stages - 1; ++i) fill(), cp_async_commit();
-    int stage = 0;
+    int slot = 0;
     const auto next = [&] {         // the next stage, whole and for all; the one behind it is filled again
         if (stages == 4) cp_async_wait<2>();
         else cp_async_wait<1>();
         __syncthreads();
         fill();
         cp_async_commit();
-        return smem + stage++ % stages * slot_bytes;
+        const unsigned char* at = smem + slot * slot_bytes;
+        if (++slot == stages) slot = 0;
+        return at;
     };
 
     // u = x A^T, a segment at a time; sums of segments join as the tree's levels complete (level l of this thread's values
