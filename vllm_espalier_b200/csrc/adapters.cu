@@ -507,21 +507,22 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
     if (ad.r8 == 0) return copy_rows<T>(p, tile_rows, mine.count, rank, CTAS, WARPS);
     const T* x = static_cast<const T*>(p.x);
     const T* y = static_cast<const T*>(p.y);
-    T* out = static_cast<T*>(p.out);
     const int K = ad.k, k_blocks = (K + 31) / 32, a_rows = ad.n_tiles * 8;
     const int blocks = block_count(p), block_lo = blocks * rank / CTAS, block_hi = blocks * (rank + 1) / CTAS;
-    const uint4 zero = {0, 0, 0, 0};
 
-    // Stages of the first product: each segment of k by itself, two blocks of 32 a stage.
+    // Stages of the first product: each segment of k by itself, two blocks of 32 a stage; of the second: four blocks of
+    // columns.
     int n_first = 0;
 #pragma unroll
     for (int s = 0; s < OWN; ++s)
         n_first += (segment_at(k_blocks, rank * OWN + s + 1) - segment_at(k_blocks, rank * OWN + s) + 1) / 2;
     const int n_second = (block_hi - block_lo + 3) / 4, n_stages = n_first + n_second;
+
     // What this thread copies of a first stage: piece tid % 8 of rows tid / 8 + 64 i of x (i = 0), then of A; of a second:
     // piece tid % 16 of rows tid / 16 + 32 i of y, then of B's. Rows of x and y that the tile lacks are left as they are (no
     // other row's result has anything of theirs).
-    constexpr int PIECES = (MANY_ROWS + MANY_COLS) * 8 / THREADS, ROW = RANK16 * 2;     // ROW: pieces of a row of B
+    constexpr int TILES = RANK16 == 1 ? 2 : RANK16 == 2 ? 4 : MANY_TILES;       // n8 tiles of the first product a warp
+    constexpr int PIECES = 1 + (TILES * 8 * 4 + MANY_ROWS - 1) / MANY_ROWS, ROW = RANK16 * 2;   // ROW: pieces of a row of B
     static_assert(MANY_ROWS * 8 == THREADS, "a piece of x a thread");
     const int piece = tid & 7, piece_row = tid >> 3;
     const T* from_first[PIECES];
@@ -537,110 +538,121 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
         const int t = tile_rows[(tid >> 4) + i * 32];
         from_y[i] = t >= 0 ? y + t * p.y_stride + (tid & 3) * 8 : nullptr;
     }
+    const uint32_t ring = smem_addr(smem), ring_end = ring + stages * slot_bytes;
     const uint32_t to_first = piece_row * 128 + (piece ^ (piece_row & 1) << 2) * 16;
     const uint32_t to_y = (tid >> 4) * 256 + ((tid & 15) ^ (tid >> 4 & 1) << 2) * 16;
-    int fill_stage = 0, fill_slot = 0, fill_segment = rank * OWN, fill_block = segment_at(k_blocks, fill_segment);
+    // The first block of a second stage, for the filling and for the use; `whole`: its four blocks are whole and of one
+    // matrix, so that their columns follow from it.
+    Block fill_at = block_lo < block_hi ? block_at(p, block_lo) : Block{0, 0, 0}, use_at = fill_at;
+    const auto whole = [&](const Block& at, int b0) { return at.left >= 128 && b0 + 4 <= block_hi; };
+    const auto advance = [&](Block& at, int b0) {       // on to block b0
+        at.col += 128, at.left -= 128;
+        if (at.left <= 0 && b0 < block_hi) at = block_at(p, b0);
+    };
+    int fill_stage = 0, fill_segment = rank * OWN, fill_block = segment_at(k_blocks, fill_segment);
     int fill_end = segment_at(k_blocks, fill_segment + 1);
+    uint32_t fill_to = ring;
     const auto fill = [&] {         // the next stage
         if (fill_stage >= n_stages) return;
-        unsigned char* to = smem + fill_slot * slot_bytes;
         if (fill_stage < n_first) {
             while (fill_block >= fill_end) fill_end = segment_at(k_blocks, ++fill_segment + 1);
             const int k = fill_block * 32;
+            const uint32_t to = fill_to + to_first;
             if (k + piece * 8 < min(fill_end * 32, K)) {
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i)
-                    if (from_first[i]) cp_async16(to + to_first + i * MANY_ROWS * 128, from_first[i] + k);
+                    if (from_first[i]) cp_async16_sa(to + i * MANY_ROWS * 128, from_first[i] + k);
             } else {
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i)
-                    if (i == 0 || from_first[i]) *reinterpret_cast<uint4*>(to + to_first + i * MANY_ROWS * 128) = zero;
+                    if (i == 0 || from_first[i]) st_shared_zero(to + i * MANY_ROWS * 128);
             }
             fill_block = min(fill_block + 2, fill_end);
         } else {
             // y: [row][16 pieces], four blocks of four
-            const int b0 = block_lo + (fill_stage - n_first) * 4, by = b0 + (tid >> 2 & 3);
-            if (by < block_hi) {
-                const Block block = block_at(p, by);
-                if ((tid & 3) * 8 < block.left)
+            const int b0 = block_lo + (fill_stage - n_first) * 4;
+            const bool all = whole(fill_at, b0);
+            const int by = tid >> 2 & 3;
+            Block block = {fill_at.m, fill_at.col + by * 32, fill_at.left - by * 32};
+            if (!all) block = b0 + by < block_hi ? block_at(p, b0 + by) : Block{0, 0, 0};
+            if ((tid & 3) * 8 < block.left)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if (from_y[i]) cp_async16(to + to_y + i * 32 * 256, from_y[i] + block.col);
-            }
+                for (int i = 0; i < 2; ++i)
+                    if (from_y[i]) cp_async16_sa(fill_to + to_y + i * 32 * 256, from_y[i] + block.col);
             // B: [block][j][g][RP]: row g of tile j is the block's column 8 (g / 2) + 2 j + g % 2
 #pragma unroll
-            for (int i = tid; i < 128 * ROW; i += THREADS) {
-                const int row = i / ROW, c = i % ROW, b = b0 + (row >> 5), j = row >> 3 & 3, gg = row & 7;
+            for (int i = 0; i < (128 * ROW + THREADS - 1) / THREADS; ++i) {
+                const int at = tid + i * THREADS, row = at / ROW, c = at % ROW, bb = row >> 5, j = row >> 3 & 3, gg = row & 7;
+                if (row >= 128) break;
                 const int n = (gg >> 1) * 8 + j * 2 + (gg & 1);
-                unsigned char* at = to + M * 256 + row * ROW * 16 + (ROW >= 8 ? c ^ (row & 1) << 2 : c) * 16;
-                if (b >= block_hi) continue;
-                const Block block = block_at(p, b);
+                const uint32_t to = fill_to + M * 256 + row * ROW * 16 + (ROW >= 8 ? c ^ (row & 1) << 2 : c) * 16;
+                block = {fill_at.m, fill_at.col + bb * 32, fill_at.left - bb * 32};
+                if (!all) block = b0 + bb < block_hi ? block_at(p, b0 + bb) : Block{0, 0, 0};
                 if (n < block.left && c * 8 < ad.r8)
-                    cp_async16(at, ad.b + (static_cast<size_t>(block.col) + n) * ad.cap + c * 8);
+                    cp_async16_sa(to, ad.b + (static_cast<size_t>(block.col) + n) * ad.cap + c * 8);
                 else
-                    *reinterpret_cast<uint4*>(at) = zero;
+                    st_shared_zero(to);
             }
+            advance(fill_at, b0 + 4);
         }
         ++fill_stage;
-        if (++fill_slot == stages) fill_slot = 0;
+        if ((fill_to += slot_bytes) == ring_end) fill_to = ring;
     };
     for (int i = 0; i < stages - 1; ++i) fill(), cp_async_commit();
-    int slot = 0;
+    uint32_t use = ring;
     const auto next = [&] {         // the next stage, whole and for all; the one behind it is filled again
         if (stages == 4) cp_async_wait<2>();
         else cp_async_wait<1>();
         __syncthreads();
         fill();
         cp_async_commit();
-        const unsigned char* at = smem + slot * slot_bytes;
-        if (++slot == stages) slot = 0;
+        const uint32_t at = use;
+        if ((use += slot_bytes) == ring_end) use = ring;
         return at;
     };
 
     // u = x A^T, a segment at a time; sums of segments join as the tree's levels complete (level l of this thread's values
     // in shared memory, where u's halves will be).
     const int per = (ad.n_tiles + 3) / 4, t0 = col_warp * per, nt = min(per, ad.n_tiles - t0);
+    const int la = row_warp * 16 + g, lb = la + 8;
     float* levels = reinterpret_cast<float*>(u.hi);
-    const auto place = [&](float* base, int j, int e) {
-        return reinterpret_cast<float2*>(
-            &base[(row_warp * 16 + g + e * 4) * cols + ad.template column<RP>(t0 + j) + q * 2]);
-    };
+    // lane (g, q)'s piece of half h of an even or odd row: q or q + 4
+    const uint32_t x_at = la * 128 + q * 16, a_at = (M + t0 * 8 + g) * 128 + q * 16, odd = (g & 1) * 64;
 #pragma unroll
     for (int s = 0; s < OWN; ++s) {
-        float acc[MANY_TILES][4] = {};
+        float acc[TILES][4] = {};
         const int end = segment_at(k_blocks, rank * OWN + s + 1);
         for (int kb = segment_at(k_blocks, rank * OWN + s); kb < end; kb += 2) {
-            const unsigned char* from = next();
+            const uint32_t from = next();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (kb + h >= end) break;
-                const auto piece = [&](int r) {
-                    return *reinterpret_cast<const uint4*>(from + r * 128 + ((h * 4 + q) ^ (r & 1) << 2) * 16);
-                };
-                const uint4 va = piece(row_warp * 16 + g), vb = piece(row_warp * 16 + g + 8);
+                const uint32_t half = h * 64 ^ odd;
+                const uint4 va = ld_shared_v4(from + x_at + half), vb = ld_shared_v4(from + x_at + half + 8 * 128);
                 const uint32_t a0[4] = {va.x, vb.x, va.y, vb.y}, a1[4] = {va.z, vb.z, va.w, vb.w};
 #pragma unroll
-                for (int j = 0; j < MANY_TILES; ++j)
+                for (int j = 0; j < TILES; ++j)
                     if (j < nt) {
-                        const uint4 w = piece(M + (t0 + j) * 8 + g);
+                        const uint4 w = ld_shared_v4(from + a_at + half + j * 8 * 128);
                         mma<T>(acc[j], a0, w.x, w.y);
                         mma<T>(acc[j], a1, w.z, w.w);
                     }
             }
         }
 #pragma unroll
-        for (int j = 0; j < MANY_TILES; ++j)
+        for (int j = 0; j < TILES; ++j)
             if (j < nt)
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
+                    const int at = (la + e * 4) * cols + ad.template column<RP>(t0 + j) + q * 2;
                     float2 v = make_float2(acc[j][e], acc[j][e + 1]);
                     int level = 0;
 #pragma unroll
-                    for (int odd = s; odd & 1; odd >>= 1, ++level) {
-                        const float2 o = *place(levels + level * M * cols, j, e);
+                    for (int bit = s; bit & 1; bit >>= 1, ++level) {
+                        const float2 o = *reinterpret_cast<const float2*>(&levels[level * M * cols + at]);
                         v.x = o.x + v.x, v.y = o.y + v.y;
                     }
-                    *place(s == OWN - 1 ? u.sums : levels + level * M * cols, j, e) = v;
+                    *reinterpret_cast<float2*>(s == OWN - 1 ? &u.sums[at] : &levels[level * M * cols + at]) = v;
                 }
     }
     cluster_sync_all();
@@ -649,33 +661,55 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
         join_row<T, RANK16, CTAS>(u, r, ad.r8, scale);
     cluster_sync_all();     // (the last access to another CTA's memory was before it)
 
-    const int la = row_warp * 16 + g, lb = la + 8, ra = tile_rows[la], rb = tile_rows[lb];
+    const int ra = tile_rows[la], rb = tile_rows[lb];
     const float fa = u.factor[la], fb = u.factor[lb];
+    T* out_a = ra >= 0 ? static_cast<T*>(p.out) + ra * p.out_stride + q * 8 : nullptr;
+    T* out_b = rb >= 0 ? static_cast<T*>(p.out) + rb * p.out_stride + q * 8 : nullptr;
+    const uint32_t y_at = la * 256 + (col_warp * 4 + q ^ (g & 1) << 2) * 16;
+    const uint32_t b_at = M * 256 + (col_warp * 32 + g) * ROW * 16;
+    const uint32_t u_at = smem_addr(u.hi + la * u.stride), lo_off = M * u.stride * sizeof(T), down = 8 * u.stride * sizeof(T);
     for (int i = 0; i < n_second; ++i) {
-        const unsigned char* from = next();
-        const int b = block_lo + i * 4 + col_warp;
-        if (b >= block_hi) continue;
-        const Block block = block_at(p, b);
-        const auto y_piece = [&](int r) {
-            return *reinterpret_cast<const uint4*>(from + r * 256 + ((col_warp * 4 + q) ^ (r & 1) << 2) * 16);
-        };
-        const unsigned char* w = from + M * 256 + (col_warp * 32 + g) * RANK16 * 32;
+        const uint32_t from = next();
+        const int b0 = block_lo + i * 4;
+        Block block = {use_at.m, use_at.col + col_warp * 32, use_at.left - col_warp * 32};
+        if (!whole(use_at, b0)) block = b0 + col_warp < block_hi ? block_at(p, b0 + col_warp) : Block{0, 0, 0};
+        advance(use_at, b0 + 4);
+        if (block.left <= 0) continue;
+        const uint32_t u_m = u_at + block.m * RP * sizeof(T);
         float acc[4][4] = {};
-        const size_t at = la * u.stride + block.m * RP;
-        second_product<T, RANK16>(acc, u.hi + at, u.lo + at, u.stride, ad.r8, q, [&](int j, int s) {
-            const unsigned char* row = w + j * 8 * RANK16 * 32;
-            if constexpr (RANK16 == 1) {
-                const uint2 v = *reinterpret_cast<const uint2*>(row + q * 8);
-                return uint4{v.x, v.y, 0, 0};
-            } else {
-                const int c = s * 2 + q;
-                return *reinterpret_cast<const uint4*>(row + (RANK16 >= 4 ? c ^ (g & 1) << 2 : c) * 16);
+        if constexpr (RANK16 == 1) {
+            const uint2 h0 = ld_shared_v2(u_m + q * 8), h1 = ld_shared_v2(u_m + down + q * 8);
+            const uint2 l0 = ld_shared_v2(u_m + lo_off + q * 8), l1 = ld_shared_v2(u_m + lo_off + down + q * 8);
+            const uint32_t hi[4] = {h0.x, h1.x, h0.y, h1.y}, lo[4] = {l0.x, l1.x, l0.y, l1.y};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint2 w = ld_shared_v2(from + b_at + j * 8 * ROW * 16 + q * 8);
+                mma<T>(acc[j], hi, w.x, w.y);
+                mma<T>(acc[j], lo, w.x, w.y);
             }
-        });
+        } else {
+#pragma unroll
+            for (int s = 0; s < RANK16; s += 2) {
+                if (s * 16 >= ad.r8) break;
+                const uint4 h0 = ld_shared_v4(u_m + s * 32 + q * 16), h1 = ld_shared_v4(u_m + down + s * 32 + q * 16);
+                const uint4 l0 = ld_shared_v4(u_m + lo_off + s * 32 + q * 16);
+                const uint4 l1 = ld_shared_v4(u_m + lo_off + down + s * 32 + q * 16);
+                const uint32_t h_a[4] = {h0.x, h1.x, h0.y, h1.y}, h_b[4] = {h0.z, h1.z, h0.w, h1.w};
+                const uint32_t l_a[4] = {l0.x, l1.x, l0.y, l1.y}, l_b[4] = {l0.z, l1.z, l0.w, l1.w};
+                const uint32_t c = RANK16 >= 4 ? (s * 2 + q ^ (g & 1) << 2) * 16 : q * 16;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 w = ld_shared_v4(from + b_at + j * 8 * ROW * 16 + c);
+                    mma<T>(acc[j], h_a, w.x, w.y);
+                    mma<T>(acc[j], l_a, w.x, w.y);
+                    mma<T>(acc[j], h_b, w.z, w.w);
+                    mma<T>(acc[j], l_b, w.z, w.w);
+                }
+            }
+        }
         if (q * 8 >= block.left) continue;
-        const int col = block.col + q * 8;
-        if (ra >= 0) *reinterpret_cast<uint4*>(out + ra * p.out_stride + col) = added<T>(y_piece(la), acc, 0, fa);
-        if (rb >= 0) *reinterpret_cast<uint4*>(out + rb * p.out_stride + col) = added<T>(y_piece(lb), acc, 2, fb);
+        if (out_a) *reinterpret_cast<uint4*>(out_a + block.col) = added<T>(ld_shared_v4(from + y_at), acc, 0, fa);
+        if (out_b) *reinterpret_cast<uint4*>(out_b + block.col) = added<T>(ld_shared_v4(from + y_at + 8 * 256), acc, 2, fb);
     }
     cp_async_wait<0>();
 }
