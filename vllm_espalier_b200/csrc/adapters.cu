@@ -58,10 +58,21 @@ __global__ void __launch_bounds__(1024) plan_kernel(AdaptParams p, Tile* tiles, 
     for (int s = tid; s < slots; s += 1024) count[s] = 0;
     if (tid == 0) base_rows = base_tiles = 0;
     __syncthreads();
-    for (int t0 = 0; t0 < p.rows; t0 += 1024) {
-        const int t = t0 + tid, id = t < p.rows ? slot_of(p, t) : -2;
-        const unsigned same = __match_any_sync(0xffffffffu, id);
-        if (id >= -1 && lane == __ffs(same) - 1) atomicAdd(&count[id < 0 ? slots - 1 : id], __popc(same));
+    // PER rows a thread at once, 1024 apart: their ids are on the way together
+    constexpr int PER = 8;
+    int ids[PER];
+    const auto load = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) ids[i] = t0 + i * 1024 + tid < p.rows ? slot_of(p, t0 + i * 1024 + tid) : -2;
+    };
+    for (int t0 = 0; t0 < p.rows; t0 += PER * 1024) {
+        load(t0);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (t0 + i * 1024 >= p.rows) break;
+            const unsigned same = __match_any_sync(0xffffffffu, ids[i]);
+            if (ids[i] >= -1 && lane == __ffs(same) - 1) atomicAdd(&count[ids[i] < 0 ? slots - 1 : ids[i]], __popc(same));
+        }
     }
     __syncthreads();
     // exclusive sums over the slots of their rows and tiles, 1024 slots a round
@@ -95,14 +106,18 @@ __global__ void __launch_bounds__(1024) plan_kernel(AdaptParams p, Tile* tiles, 
         __syncthreads();
     }
     for (int i = base_tiles + tid; i < p.max_tiles; i += 1024) tiles[i] = {-1, 0, 0, 0};
-    for (int t0 = 0; t0 < p.rows; t0 += 1024) {
-        const int t = t0 + tid, id = t < p.rows ? slot_of(p, t) : -2;
-        const unsigned same = __match_any_sync(0xffffffffu, id);
-        const int leader = __ffs(same) - 1;
-        int at = 0;
-        if (id >= -1 && lane == leader) at = atomicAdd(&count[id < 0 ? slots - 1 : id], __popc(same));
-        at = __shfl_sync(0xffffffffu, at, leader);
-        if (id >= -1) rows[at + __popc(same & ((1u << lane) - 1))] = t;
+    for (int t0 = 0; t0 < p.rows; t0 += PER * 1024) {
+        if (p.rows > PER * 1024) load(t0);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (t0 + i * 1024 >= p.rows) break;
+            const unsigned same = __match_any_sync(0xffffffffu, ids[i]);
+            const int leader = __ffs(same) - 1;
+            int at = 0;
+            if (ids[i] >= -1 && lane == leader) at = atomicAdd(&count[ids[i] < 0 ? slots - 1 : ids[i]], __popc(same));
+            at = __shfl_sync(0xffffffffu, at, leader);
+            if (ids[i] >= -1) rows[at + __popc(same & ((1u << lane) - 1))] = t0 + i * 1024 + tid;
+        }
     }
 }
 
@@ -630,13 +645,16 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
                 const uint32_t half = h * 64 ^ odd;
                 const uint4 va = ld_shared_v4(from + x_at + half), vb = ld_shared_v4(from + x_at + half + 8 * 128);
                 const uint32_t a0[4] = {va.x, vb.x, va.y, vb.y}, a1[4] = {va.z, vb.z, va.w, vb.w};
+                uint4 w[TILES];
 #pragma unroll
                 for (int j = 0; j < TILES; ++j)
-                    if (j < nt) {
-                        const uint4 w = ld_shared_v4(from + a_at + half + j * 8 * 128);
-                        mma<T>(acc[j], a0, w.x, w.y);
-                        mma<T>(acc[j], a1, w.z, w.w);
-                    }
+                    if (j < nt) w[j] = ld_shared_v4(from + a_at + half + j * 8 * 128);
+#pragma unroll
+                for (int j = 0; j < TILES; ++j)
+                    if (j < nt) mma<T>(acc[j], a0, w[j].x, w[j].y);
+#pragma unroll
+                for (int j = 0; j < TILES; ++j)
+                    if (j < nt) mma<T>(acc[j], a1, w[j].z, w[j].w);
             }
         }
 #pragma unroll
@@ -681,12 +699,13 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
             const uint2 h0 = ld_shared_v2(u_m + q * 8), h1 = ld_shared_v2(u_m + down + q * 8);
             const uint2 l0 = ld_shared_v2(u_m + lo_off + q * 8), l1 = ld_shared_v2(u_m + lo_off + down + q * 8);
             const uint32_t hi[4] = {h0.x, h1.x, h0.y, h1.y}, lo[4] = {l0.x, l1.x, l0.y, l1.y};
+            uint2 w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint2 w = ld_shared_v2(from + b_at + j * 8 * ROW * 16 + q * 8);
-                mma<T>(acc[j], hi, w.x, w.y);
-                mma<T>(acc[j], lo, w.x, w.y);
-            }
+            for (int j = 0; j < 4; ++j) w[j] = ld_shared_v2(from + b_at + j * 8 * ROW * 16 + q * 8);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma<T>(acc[j], hi, w[j].x, w[j].y);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma<T>(acc[j], lo, w[j].x, w[j].y);
         } else {
 #pragma unroll
             for (int s = 0; s < RANK16; s += 2) {
@@ -697,14 +716,17 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
                 const uint32_t h_a[4] = {h0.x, h1.x, h0.y, h1.y}, h_b[4] = {h0.z, h1.z, h0.w, h1.w};
                 const uint32_t l_a[4] = {l0.x, l1.x, l0.y, l1.y}, l_b[4] = {l0.z, l1.z, l0.w, l1.w};
                 const uint32_t c = RANK16 >= 4 ? (s * 2 + q ^ (g & 1) << 2) * 16 : q * 16;
+                uint4 w[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint4 w = ld_shared_v4(from + b_at + j * 8 * ROW * 16 + c);
-                    mma<T>(acc[j], h_a, w.x, w.y);
-                    mma<T>(acc[j], l_a, w.x, w.y);
-                    mma<T>(acc[j], h_b, w.z, w.w);
-                    mma<T>(acc[j], l_b, w.z, w.w);
-                }
+                for (int j = 0; j < 4; ++j) w[j] = ld_shared_v4(from + b_at + j * 8 * ROW * 16 + c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma<T>(acc[j], h_a, w[j].x, w[j].y);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma<T>(acc[j], l_a, w[j].x, w[j].y);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma<T>(acc[j], h_b, w[j].z, w[j].w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma<T>(acc[j], l_b, w[j].z, w[j].w);
             }
         }
         if (q * 8 >= block.left) continue;
@@ -798,12 +820,15 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
             return rc;
         return ok();
     }
-    // CTAs a tile: as few as fill the GPU's places (two CTAs an SM, one from rank 33 on) in the fewest rounds of work.
-    const int places = device_sms() * (steps >= 4 ? 1 : 2), tiles = (t_rows + m - 1) / m + std::min(ad->slots, t_rows / m) / 2;
-    int ctas = 8;
+    // CTAs a tile: what takes the least rounds x (a CTA's share of a tile + what it spends on joining sums). Places: two CTAs
+    // an SM (one from rank 33 on), as many whole clusters as the 18 SMs of a GPC hold. Measured: 128 tiles of rank 16 with 2 /
+    // 4 / 8 CTAs 68 / 74 / 90 us, 47 tiles of rank 64 with 4 / 8 75 / 85 us.
+    const int an_sm = steps >= 4 ? 1 : 2, tiles = (t_rows + m - 1) / m + std::min(ad->slots, t_rows / m) / 2;
+    int ctas = 8;       // (fits whatever fits at all)
     double best = 1e30;
     for (int c : {2, 4, 8}) {
         if (many_bytes(cols, steps, 3, c) > MAX_SMEM) continue;
+        const int places = std::max(device_sms() / 18, 1) * (18 * an_sm / c) * c;
         const double work = ((tiles * c + places - 1) / places) * (1.0 / c + CTA_COST);
         if (work < best) best = work, ctas = c;
     }
