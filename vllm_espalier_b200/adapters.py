@@ -14,10 +14,11 @@ import ctypes as C
 
 import torch
 
-from ._lib import DTYPE, check, esp_adapters_t, lib, ptr, stream_ptr
+from ._lib import DTYPE, check, esp_adapters_t, lib, stream_ptr
 
 MAX_RANK, MAX_MATS, MAX_SLOTS = 128, 4, 4096
 NONE = -1                     # the id of a row without an adapter
+NO_PLAN = 64                  # rows up to which the kernel takes no workspace
 
 
 class Adapters:
@@ -107,38 +108,42 @@ class Adapters:
         self.a[slot].zero_()
         self.b[slot].zero_()
 
-    def _rows(self, t: torch.Tensor, name: str, columns: int) -> torch.Tensor:
-        if t.dim() != 2 or t.shape[1] != columns or t.dtype != self.dtype or t.device != self.device:
+    def _rows(self, t: torch.Tensor, name: str, columns: int) -> tuple[int, bool]:
+        """(row stride, whether the kernel takes the rows as they are: unit columns, 16-byte aligned)."""
+        if t.dtype != self.dtype or t.dim() != 2 or t.shape[1] != columns or t.device != self.device:
             raise ValueError(f"{name} must be {self.dtype} [rows, {columns}] on {self.device}, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
-        return t
-
-    @staticmethod
-    def _aligned(t: torch.Tensor) -> bool:
-        return t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+        stride, step = t.stride()
+        return stride, step == 1 and not stride & 7 and not t.data_ptr() & 15
 
     def forward(self, x: torch.Tensor, y: torch.Tensor, ids: torch.Tensor, out: torch.Tensor | None = None):
         """x [rows, k], y [rows, sum(widths)] in the adapters' dtype, ids int32 [rows] (outside [0, slots): no adapter).
         Returns out (a new tensor, or the one given: y itself adds in place)."""
-        x, y = self._rows(x, "x", self.k), self._rows(y, "y", self.n)
+        (x_stride, x_fits), (y_stride, y_fits) = self._rows(x, "x", self.k), self._rows(y, "y", self.n)
         rows = x.shape[0]
-        if y.shape[0] != rows or ids.shape != (rows,):
+        if y.shape[0] != rows or ids.dim() != 1 or ids.numel() != rows:
             raise ValueError(f"x has {rows} rows, y {y.shape[0]}, ids {tuple(ids.shape)}")
         if ids.dtype != torch.int32 or ids.device != self.device or not ids.is_contiguous():
             raise ValueError(f"ids must be contiguous int32 on {self.device}, got {ids.dtype} on {ids.device}")
         if out is None:
-            out = torch.empty((rows, self.n), dtype=self.dtype, device=self.device)
-        elif self._rows(out, "out", self.n).shape[0] != rows or (rows and not self._aligned(out)):
-            raise ValueError(f"out must be [{rows}, {self.n}] with 16-byte aligned rows and unit column stride")
+            out, out_stride = y.new_empty((rows, self.n)), self.n
+        else:
+            out_stride, fits = self._rows(out, "out", self.n)
+            if out.shape[0] != rows or (rows and not fits):
+                raise ValueError(f"out must be [{rows}, {self.n}] with 16-byte aligned rows and unit column stride")
         if not rows:
             return out
-        x = x if self._aligned(x) else x.clone(memory_format=torch.contiguous_format)
-        y = y if self._aligned(y) else y.clone(memory_format=torch.contiguous_format)
-        need, ws = lib().esp_adapt_ws_bytes(rows, self.slots), None
-        if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        check(lib().esp_adapt(self._ref, x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), ids.data_ptr(), rows,
-                              out.data_ptr(), out.stride(0), ptr(ws), need, stream_ptr(self.device)))
+        if not x_fits:
+            x, x_stride = x.clone(memory_format=torch.contiguous_format), self.k
+        if not y_fits:
+            y, y_stride = y.clone(memory_format=torch.contiguous_format), self.n
+        need = ws = 0
+        if rows > NO_PLAN:
+            need = lib().esp_adapt_ws_bytes(rows, self.slots)
+            scratch = ids.new_empty((need + 3) // 4)
+            ws = scratch.data_ptr()
+        check(lib().esp_adapt(self._ref, x.data_ptr(), x_stride, y.data_ptr(), y_stride, ids.data_ptr(), rows,
+                              out.data_ptr(), out_stride, ws, need, stream_ptr(self.device)))
         return out
 
     __call__ = forward

@@ -83,4 +83,13 @@ int allow_smem(K kernel, size_t bytes) {
     return ESP_OK;
 }
 
+// Opt a kernel into clusters of more than eight CTAs.
+template <typename K>
+int allow_cluster16(K kernel) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return set_error(ESP_ERR_CUDA, "cluster size opt-in: %s", cudaGetErrorString(e));
+    return ESP_OK;
+}
+
 }  // namespace esp

@@ -596,8 +596,8 @@ extern "C" int esp_verify(const void* logits, int dtype, long long stride, long 
     while (1 << log2 < segments && (static_cast<long long>(requests) << log2) < FILL * sms) ++log2;
     const int ctas = 1 << log2;
     ESP_REQUIRE(requests <= INT_MAX >> log2, ESP_ERR_INVALID, "esp_verify: %d requests", requests);
-    if (ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-        return cuda_status("esp_verify: cluster of 16");
+    if (ctas > 8)
+        if (const int rc = allow_cluster16(kernel)) return rc;
     const Split split{log2, segments, segments >> log2, (vocab + 8 * segments - 1) / (8 * segments) * 8,
                       requests * ctas <= sms};
     if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(requests) << log2), dim3(THREADS), 0, stream, true,

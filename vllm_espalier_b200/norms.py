@@ -107,13 +107,13 @@ class BlockNorm:
                 raise ValueError(f"gate must be [{d}], [{rows}, 1] or [{rows}, {d}], got {tuple(gate.shape)}")
             gate_ptr, gate_dtype = gate.data_ptr(), DTYPE[gate.dtype]
         if out is None:
-            out, r_stride = torch.empty_like(r_like, memory_format=torch.contiguous_format), d
+            out, r_stride = r_like.new_empty((rows, d)), d
         else:
             r_stride = self._given(out, "out", x, r_dtype)
         h_ptr = h_stride = 0
         if self.has_pre:
             if normed is None:
-                normed, h_stride = torch.empty_like(x, memory_format=torch.contiguous_format), d
+                normed, h_stride = x.new_empty((rows, d)), d
             else:
                 h_stride = self._given(normed, "normed", x, x_dtype)
             h_ptr = normed.data_ptr()

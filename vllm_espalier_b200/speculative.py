@@ -15,14 +15,6 @@ import torch
 from ._lib import DTYPE, check, lib, stream_ptr
 
 
-def _flat(t: torch.Tensor, n: int, dtype: torch.dtype, name: str, dev) -> int:
-    if t.shape != (n,) or t.dtype != dtype or t.device != dev:
-        raise ValueError(f"{name} must be {dtype} [{n}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
-
-
 def verify(logits: torch.Tensor, starts: torch.Tensor, drafts: torch.Tensor, uniform: torch.Tensor,
            noise: torch.Tensor, max_drafts: int, temperature: torch.Tensor | None = None,
            draft_probs: torch.Tensor | None = None):
@@ -34,44 +26,51 @@ def verify(logits: torch.Tensor, starts: torch.Tensor, drafts: torch.Tensor, uni
 
     Returns (tokens int32 [B, max_drafts + 1], accepted int32 [B], probs fp32 [B, max_drafts + 1]): the drafted tokens
     that stand and the drawn one, then -1; how many stand; the target's probability of each token (0 at -1)."""
-    if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in DTYPE:
+    code = DTYPE.get(logits.dtype)
+    if code is None or logits.dim() != 2 or not logits.is_cuda:
         raise ValueError(f"logits must be a CUDA fp16/bf16/fp32 [rows, vocab] tensor, got {logits.dtype} "
                          f"{tuple(logits.shape)}")
     dev, (rows, vocab) = logits.device, logits.shape
-    if starts.dim() != 1 or starts.shape[0] < 1:
+    if starts.dim() != 1 or starts.numel() < 1:
         raise ValueError(f"starts must be int32 [requests + 1], got {tuple(starts.shape)}")
-    B = starts.shape[0] - 1
+    B = starts.numel() - 1
     n = rows - B
     if n < 0 or (B == 0 and n > 0):
         raise ValueError(f"{rows} rows of logits for {B} requests: every request has a row for each drafted token "
                          "and one more")
     if vocab < 1 or max_drafts < 0:
         raise ValueError(f"a vocabulary of {vocab} and at most {max_drafts} drafted tokens")
-    if logits.stride(1) != 1:
-        logits = logits.contiguous()
-    at = [_flat(starts, B + 1, torch.int32, "starts", dev), _flat(drafts, n, torch.int32, "drafts", dev),
-          _flat(uniform, n, torch.float32, "uniform", dev)]
-    if noise.shape != (B, vocab) or noise.dtype != torch.float32 or noise.device != dev:
+    flat = [("starts", starts, B + 1, torch.int32), ("drafts", drafts, n, torch.int32),
+            ("uniform", uniform, n, torch.float32)]
+    if temperature is not None:
+        flat.append(("temperature", temperature, B, torch.float32))
+    at = []
+    for name, t, size, dtype in flat:
+        if t.dtype != dtype or t.dim() != 1 or t.numel() != size or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {dtype} [{size}] on {dev}, got {t.dtype} {tuple(t.shape)} on "
+                             f"{t.device}")
+        at.append(t.data_ptr())
+    if noise.dtype != torch.float32 or noise.shape != (B, vocab) or noise.device != dev:
         raise ValueError(f"noise must be fp32 [{B}, {vocab}] on {dev}, got {noise.dtype} {tuple(noise.shape)} on "
                          f"{noise.device}")
-    if noise.stride(1) != 1:
-        noise = noise.contiguous()
-    t_ptr = q_ptr = q_stride = q_dtype = 0
-    if temperature is not None:
-        t_ptr = _flat(temperature, B, torch.float32, "temperature", dev)
+    (stride, step), (noise_stride, noise_step) = logits.stride(), noise.stride()
+    if step != 1:
+        logits, stride = logits.contiguous(), vocab
+    if noise_step != 1:
+        noise, noise_stride = noise.contiguous(), vocab
+    q_ptr = q_stride = q_code = 0
     if draft_probs is not None:
-        if draft_probs.shape != (n, vocab) or draft_probs.dtype not in DTYPE or draft_probs.device != dev:
+        q_code = DTYPE.get(draft_probs.dtype)
+        if q_code is None or draft_probs.shape != (n, vocab) or draft_probs.device != dev:
             raise ValueError(f"draft_probs must be fp16/bf16/fp32 [{n}, {vocab}] on {dev}, got {draft_probs.dtype} "
                              f"{tuple(draft_probs.shape)} on {draft_probs.device}")
         if draft_probs.stride(1) != 1:
             draft_probs = draft_probs.contiguous()
-        q_ptr, q_stride, q_dtype = draft_probs.data_ptr(), draft_probs.stride(0), DTYPE[draft_probs.dtype]
-    tokens = torch.empty((B, max_drafts + 1), dtype=torch.int32, device=dev)
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    probs = torch.empty((B, max_drafts + 1), dtype=torch.float32, device=dev)
+        q_ptr, q_stride = draft_probs.data_ptr(), draft_probs.stride(0)
+    tokens = starts.new_empty((B, max_drafts + 1))      # int32; new_empty parses no options
+    accepted, probs = starts.new_empty(B), noise.new_empty((B, max_drafts + 1))
     if B:
-        check(lib().esp_verify(logits.data_ptr(), DTYPE[logits.dtype], logits.stride(0), rows, vocab, at[0], B, at[1],
-                               at[2], n, q_ptr, q_dtype, q_stride, noise.data_ptr(), noise.stride(0), t_ptr,
-                               int(max_drafts), tokens.data_ptr(), accepted.data_ptr(), probs.data_ptr(),
-                               stream_ptr(dev)))
+        check(lib().esp_verify(logits.data_ptr(), code, stride, rows, vocab, at[0], B, at[1], at[2], n, q_ptr, q_code,
+                               q_stride, noise.data_ptr(), noise_stride, at[3] if len(at) > 3 else 0, max_drafts,
+                               tokens.data_ptr(), accepted.data_ptr(), probs.data_ptr(), stream_ptr(dev)))
     return tokens, accepted, probs
