@@ -187,6 +187,36 @@ def test_strided_rows_and_outputs_in_place(dev, d, pad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [1, 2, 3, 7, 8, 9, 15, 17, 31, 250, 257, 263, 1016, 1023, 1025, 2047, 2049, 4095, 8191])
+@pytest.mark.parametrize("off,pad", [(0, 1), (1, 0), (3, 2), (5, 5), (6, 1), (7, 0)])
+def test_any_alignment(dev, dtype, d, off, pad):
+    """16-bit rows that start on any 2-byte boundary, outputs into buffers whose other values stay, and in place."""
+    rows = 4
+    t = inputs(dev, rows, d, dtype, dtype, True, "element", True, 11)
+
+    def inside(v, o, fill=float("nan")):
+        wide = torch.full((rows, d + off + pad + 8), fill, dtype=dtype, device=dev)
+        if v is not None:
+            wide[:, o:o + d] = v
+        return wide, wide[:, o:o + d]
+    op = norms.BlockNorm(d, pre=t["pre"], pre_bias=t["pre_bias"], post=t["post"], post_bias=t["post_bias"],
+                         kind="layer", eps=EPS, gate_act="sigmoid", residual_scale=0.9, block_scale=1.25)
+    x, residual = inside(t["x"], off)[1], inside(t["residual"], pad)[1]
+    x2, gate = inside(t["x2"], off + 1)[1], inside(t["gate"], pad + 2)[1]
+    (wide_r, r), (wide_h, h) = inside(None, off + 2, 7.0), inside(None, pad + 1, 7.0)
+    op(x, residual, x2=x2, gate=gate, out=r, normed=h)
+    want = reference("layer", "sigmoid", 0.9, 1.25, 0.0, use_post=True, **t)
+    check(r, want[0], want[1])
+    check(h, want[2], want[3])
+    for wide, o in ((wide_r, off + 2), (wide_h, pad + 1)):
+        assert (wide[:, :o] == 7).all() and (wide[:, o + d:] == 7).all()
+    r0, h0 = r.clone(), h.clone()
+    op(x, residual, x2=x2, gate=gate, out=residual, normed=x)
+    assert torch.equal(residual, r0) and torch.equal(x, h0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d", [2048, 1023])
 def test_rows_do_not_touch_each_other(dev, d):
     """A row's bits do not depend on the others, be they NaN, and not on how many there are."""

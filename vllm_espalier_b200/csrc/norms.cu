@@ -147,6 +147,67 @@ __device__ __forceinline__ void fetch(Group<T, VEC>& g, const void* base, size_t
     g = *reinterpret_cast<const Group<T, VEC>*>(static_cast<const T*>(base) + i);
 }
 
+// Eight 16-bit values from any 2-byte boundary on, `n` of them the row's (the rest come out as anything): the 16-byte blocks
+// that hold them (each has a byte of the row, so it is mapped memory) and a shift, the same for all of a row's groups.
+template <typename T>
+__device__ __forceinline__ void fetch_shifted(Group<T, 8>& g, const void* base, size_t i, int n) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(static_cast<const T*>(base) + i);
+    const int s = a % 16;
+    const uint4* from = reinterpret_cast<const uint4*>(a - s);
+    uint4 lo = from[0], hi = {0, 0, 0, 0};
+    if (s && 16 < s + 2 * n) hi = from[1];
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (s & 4)
+#pragma unroll
+        for (int k = 0; k < 7; ++k) w[k] = w[k + 1];
+    if (s & 8)
+#pragma unroll
+        for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+    if (s & 2)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+    g = *reinterpret_cast<const Group<T, 8>*>(w);
+}
+
+// The other way round, by all lanes of a warp with consecutive groups (n <= 0: none): a lane stores the 16-byte block in
+// which its group starts, with the end of the group before it from its neighbour; at the ends of the warp and of the row
+// the pieces of a block go one by one.
+template <typename T>
+__device__ __forceinline__ void store_shifted(const Group<T, 8>& g, void* base, size_t i, int n) {
+    T* to = static_cast<T*>(base) + i;
+    const int s = reinterpret_cast<uintptr_t>(to) % 16, lane = threadIdx.x & 31, first = (16 - s) / 2;   // of the group's in its block
+    const uint32_t* o = reinterpret_cast<const uint32_t*>(&g);
+    uint32_t w[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = __shfl_up_sync(0xffffffffu, o[k], 1), w[k + 4] = o[k];
+    const int next = __shfl_down_sync(0xffffffffu, n, 1);
+    if (n <= 0) return;
+    const bool block = s == 0 ? n == 8 : lane > 0 && n >= first;
+    if (block) {
+        const int skip = 16 - s;        // bytes of the two groups before the block
+        if (s == 0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = w[k + 4];
+        } else {
+            if (skip & 4)
+#pragma unroll
+                for (int k = 0; k < 7; ++k) w[k] = w[k + 1];
+            if (skip & 8)
+#pragma unroll
+                for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+            if (skip & 2)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+        }
+        *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(to) - s) = {w[0], w[1], w[2], w[3]};
+    }
+    // one by one: what is before the next block where this lane stored none, and what is in it where no lane stores that
+    const bool followed = lane < 31 && next >= first;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n && (e < first ? !block : !followed)) to[e] = g.e[e];
+}
+
 // The sum over the CTA with one barrier; `scratch` (a word a warp) is this reduction's own.
 template <int NT>
 __device__ __forceinline__ float rows_sum(float v, float* scratch) {
@@ -164,6 +225,24 @@ __device__ __forceinline__ float rows_sum(float v, float* scratch) {
     return (s.x + s.y) + (s.z + s.w);
 }
 
+template <bool SHIFT, typename T, int VEC>
+__device__ __forceinline__ void fetch_any(Group<T, VEC>& g, const void* base, int c, int d) {
+    if constexpr (SHIFT) {
+        if (c < d) fetch_shifted(g, base, c, d - c);
+    } else {
+        fetch(g, base, c);
+    }
+}
+
+// A group's values from the n-th on become 0.
+template <int VEC>
+__device__ __forceinline__ void zero_from(float (&v)[VEC], int n) {
+    if (n < VEC)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (e >= n) v[e] = 0.0f;
+}
+
 // v becomes (v - mean) for a layer norm; inv the reciprocal root of its second moment. Columns past d hold 0 in v.
 template <int NT, int VEC, int VPT>
 __device__ __forceinline__ float rows_moments(float (&v)[VPT][VEC], int d, int kind, float eps, float (*scratch)[32]) {
@@ -176,9 +255,11 @@ __device__ __forceinline__ float rows_moments(float (&v)[VPT][VEC], int d, int k
         const float mean = rows_sum<NT>(s, scratch[0]) / d;
 #pragma unroll
         for (int j = 0; j < VPT; ++j)
-            if ((j * NT + static_cast<int>(threadIdx.x)) * VEC < d)
+            if ((j * NT + static_cast<int>(threadIdx.x)) * VEC < d) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[j][e] -= mean;
+                if (VEC > 1) zero_from(v[j], d - (j * NT + static_cast<int>(threadIdx.x)) * VEC);
+            }
     }
     float q = 0.0f;
 #pragma unroll
@@ -243,7 +324,7 @@ __device__ __forceinline__ void fetch_weights(RowWeights<TW, VEC, VPT>& w, const
 
 // Row t from its inputs to its outputs. Each term is a branch of the whole group, not of each value. WEIGHTS: the weights
 // are in `w`, otherwise they are read where they are used.
-template <typename TX, typename TR, typename TW, int VEC, int NT, int VPT, bool WEIGHTS, typename In>
+template <typename TX, typename TR, typename TW, int VEC, int NT, int VPT, bool WEIGHTS, bool SHIFT = false, typename In>
 __device__ __forceinline__ void norm_row(const NormParams& p, size_t t, const In& in, RowWeights<TW, VEC, VPT>& w,
                                          float (*scratch)[32]) {
     const int d = p.op.d;
@@ -262,6 +343,7 @@ __device__ __forceinline__ void norm_row(const NormParams& p, size_t t, const In
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[j][e] += f32(x2.e[e]);
             }
+            if (SHIFT) zero_from(v[j], d - c);
         } else {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[j][e] = 0.0f;
@@ -271,7 +353,7 @@ __device__ __forceinline__ void norm_row(const NormParams& p, size_t t, const In
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int c = (j * NT + static_cast<int>(threadIdx.x)) * VEC;
-        if (c >= d) continue;
+        if (!SHIFT && c >= d) continue;
         float(&a)[VEC] = v[j];
         if (p.op.post)
 #pragma unroll
@@ -282,7 +364,7 @@ __device__ __forceinline__ void norm_row(const NormParams& p, size_t t, const In
         }
         if (p.op.post_b) {
             Group<TW, VEC> b;
-            fetch(b, p.op.post_b, c);
+            fetch_any<SHIFT>(b, p.op.post_b, c, d);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) a[e] += f32(b.e[e]);
         }
@@ -304,10 +386,12 @@ __device__ __forceinline__ void norm_row(const NormParams& p, size_t t, const In
 #pragma unroll
             for (int e = 0; e < VEC; ++e) a[e] = fmaf(p.op.residual_scale, f32(res.e[e]), a[e]);
         }
+        if (SHIFT) zero_from(a, d - c);
         if (p.r_out) {
             Group<TR, VEC> r;
             rounded(a, r);
-            *reinterpret_cast<Group<TR, VEC>*>(static_cast<TR*>(p.r_out) + t * p.r_out_stride + c) = r;
+            if constexpr (SHIFT) store_shifted(r, p.r_out, t * p.r_out_stride + c, min(8, d - c));
+            else *reinterpret_cast<Group<TR, VEC>*>(static_cast<TR*>(p.r_out) + t * p.r_out_stride + c) = r;
         }
     }
     if (!p.op.pre) return;
@@ -315,7 +399,7 @@ __device__ __forceinline__ void norm_row(const NormParams& p, size_t t, const In
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int c = (j * NT + static_cast<int>(threadIdx.x)) * VEC;
-        if (c >= d) continue;
+        if (!SHIFT && c >= d) continue;
         float(&a)[VEC] = v[j];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) a[e] *= inv2;
@@ -325,13 +409,14 @@ __device__ __forceinline__ void norm_row(const NormParams& p, size_t t, const In
         }
         if (p.op.pre_b) {
             Group<TW, VEC> b;
-            fetch(b, p.op.pre_b, c);
+            fetch_any<SHIFT>(b, p.op.pre_b, c, d);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) a[e] += f32(b.e[e]);
         }
         Group<TX, VEC> h;
         rounded(a, h);
-        *reinterpret_cast<Group<TX, VEC>*>(static_cast<TX*>(p.h_out) + t * p.h_out_stride + c) = h;
+        if constexpr (SHIFT) store_shifted(h, p.h_out, t * p.h_out_stride + c, min(8, d - c));
+        else *reinterpret_cast<Group<TX, VEC>*>(static_cast<TX*>(p.h_out) + t * p.h_out_stride + c) = h;
     }
 }
 
@@ -355,6 +440,28 @@ __global__ void __launch_bounds__(NT) block_norm_rows(NormParams p) {
     }
     if constexpr (VEC > 1) fetch_weights<TW, VEC, NT, VPT>(w, p);
     norm_row<TX, TR, TW, VEC, NT, VPT, (VEC > 1)>(p, t, in, w, scratch);
+}
+
+// 16-bit rows of any width and alignment by 16-byte loads and stores all the same: each group of eight shifted into place.
+// Same columns a thread as block_norm_rows with VEC 8.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) block_norm_shifted(NormParams p) {
+    __shared__ __align__(16) float scratch[4][32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const size_t t = blockIdx.x;
+    InRegisters<T, T, 8, 1> in;
+    RowWeights<T, 8, 1> w;
+    const int c = threadIdx.x * 8, n = p.op.d - c;
+    if (n > 0) {
+        fetch_shifted(in.x_[0], p.x, t * p.x_stride + c, n);
+        if (p.x2) fetch_shifted(in.x2_[0], p.x2, t * p.x2_stride + c, n);
+        if (p.residual) fetch_shifted(in.res_[0], p.residual, t * p.residual_stride + c, n);
+        if (gated(p)) fetch_shifted(in.gate_[0], p.gate, (p.gate_kind == ESP_GATE_ELEMENT ? t * p.gate_stride : 0) + c, n);
+        if (p.op.post_w) fetch_shifted(w.post_w[0], p.op.post_w, c, n);
+        if (p.op.pre_w) fetch_shifted(w.pre_w[0], p.op.pre_w, c, n);
+    }
+    norm_row<T, T, T, 8, NT, 1, true, true>(p, t, in, w, scratch);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -458,7 +565,13 @@ RowsKernel rows_kernel(int d, bool vec) {
         if (d <= 8192) return rows_instance<TX, TR, TW, 8, 512, 2>();
         return {};
     }
-    if (d <= 2048) return rows_instance<TX, TR, TW, 1, 256, 8>();
+    if constexpr (sizeof(TX) == 2 && std::is_same_v<TX, TR> && std::is_same_v<TX, TW>) {
+        if (d <= 1024) return {block_norm_shifted<TX, 128>, nullptr, 128, 0};
+        if (d <= 2048) return {block_norm_shifted<TX, 256>, nullptr, 256, 0};
+        if (d <= 4096) return {block_norm_shifted<TX, 512>, nullptr, 512, 0};
+        if (d <= 8192) return {block_norm_shifted<TX, 1024>, nullptr, 1024, 0};
+    }
+    if (d <= 2048) return rows_instance<TX, TR, TW, 1, 512, 4>();
     if (d <= 8192) return rows_instance<TX, TR, TW, 1, 1024, 8>();
     return {};
 }
