@@ -33,7 +33,7 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-constexpr int THREADS = 256, WARPS = THREADS / 32, PACKS = 4, OCTETS = 2, SINGLES = 8, RESIDENT = 4;
+constexpr int THREADS = 256, WARPS = THREADS / 32, PACKS = 4, OCTETS = 1, SINGLES = 8, RESIDENT = 4;
 constexpr int MAX_SEGMENTS = 16, SEGMENT = 16384, FILL = 4;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -223,14 +223,14 @@ __device__ __forceinline__ Part fast_part(const T* row, int lo, int hi, float c)
         if (l > m) raise(l, v);
         z += ex2(fmaf(l, c, -mc));
     };
-    // PACKS packs, THREADS apart, from pack i on; those past the end read as the batch's first once more and weigh nothing
-    const auto batch = [&](int i, auto whole) {
-        Pack<T> k[PACKS];
+    // PACKS packs, THREADS apart, from pack i on; those past the end read as the batch's first once more and weigh nothing.
+    // The next batch is on its way while one is used.
+    const auto load = [&](Pack<T> (&k)[PACKS], int i) {
 #pragma unroll
-        for (int u = 0; u < PACKS; ++u) {
-            const bool in = whole || u == 0 || i + u * THREADS < packs;
-            k[u] = *reinterpret_cast<const Pack<T>*>(row + head + (in ? i + u * THREADS : i) * N);
-        }
+        for (int u = 0; u < PACKS; ++u)
+            k[u] = *reinterpret_cast<const Pack<T>*>(row + head + (u == 0 || i + u * THREADS < packs ? i + u * THREADS : i) * N);
+    };
+    const auto use = [&](const Pack<T> (&k)[PACKS], int i, auto whole) {
         const float top = largest_of(k);
         if (top > m) raise(top, head + i * N);
 #pragma unroll
@@ -242,8 +242,18 @@ __device__ __forceinline__ Part fast_part(const T* row, int lo, int hi, float c)
     // before the packs, so that a thread meets its places in order
     if (lo + static_cast<int>(threadIdx.x) < head) single(lo + threadIdx.x);
     int i = threadIdx.x;
-    for (; i + (PACKS - 1) * THREADS < packs; i += PACKS * THREADS) batch(i, std::true_type());
-    if (i < packs) batch(i, std::false_type());
+    if (i < packs) {
+        Pack<T> k[PACKS], then[PACKS];
+        load(k, i);
+        while (i + PACKS * THREADS < packs) {
+            load(then, i + PACKS * THREADS);
+            use(k, i, std::true_type());
+#pragma unroll
+            for (int u = 0; u < PACKS; ++u) k[u] = then[u];
+            i += PACKS * THREADS;
+        }
+        use(k, i, std::false_type());
+    }
     if (tail + static_cast<int>(threadIdx.x) < hi) single(tail + threadIdx.x);
     if (first >= 0) z *= ex2(-fmaf(m, c, -mc));
     return {m, z, first < 0 ? INT_MAX : first, 0};
@@ -349,25 +359,29 @@ __device__ __forceinline__ void race(Best& best, const T* row, const Q* q, const
     if ((reinterpret_cast<uintptr_t>(row + lo) | reinterpret_cast<uintptr_t>(noise + lo) |
          (SUBTRACT ? reinterpret_cast<uintptr_t>(q) + lo * sizeof(O) : 0)) % 16 == 0) {
         const int groups = (hi - lo) / 8;
-        const auto batch = [&](int g, auto whole) {
+        struct Octets {
             Octet<T> l[OCTETS];
             Octet<float> e[OCTETS];
-            [[maybe_unused]] Octet<O> o[OCTETS];
+            Octet<O> o[SUBTRACT ? OCTETS : 1];
+        };
+        const auto load = [&](Octets& k, int g) {
 #pragma unroll
             for (int u = 0; u < OCTETS; ++u) {
-                const int at = lo + (whole || g + u * THREADS < groups ? g + u * THREADS : g) * 8;
-                l[u] = *reinterpret_cast<const Octet<T>*>(row + at);
-                e[u] = *reinterpret_cast<const Octet<float>*>(noise + at);
-                if constexpr (SUBTRACT) o[u] = *reinterpret_cast<const Octet<O>*>(q + at);
+                const int at = lo + (u == 0 || g + u * THREADS < groups ? g + u * THREADS : g) * 8;
+                k.l[u] = *reinterpret_cast<const Octet<T>*>(row + at);
+                k.e[u] = *reinterpret_cast<const Octet<float>*>(noise + at);
+                if constexpr (SUBTRACT) k.o[u] = *reinterpret_cast<const Octet<O>*>(q + at);
             }
+        };
+        const auto use = [&](const Octets& k, int g) {
 #pragma unroll
             for (int u = 0; u < OCTETS; ++u) {
-                const int at = lo + (whole || g + u * THREADS < groups ? g + u * THREADS : g) * 8;
+                const int at = lo + (u == 0 || g + u * THREADS < groups ? g + u * THREADS : g) * 8;
                 float s[8], top = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if constexpr (SUBTRACT) s[j] = score(l[u].e[j], e[u].e[j], f32(o[u].e[j]));
-                    else s[j] = score(l[u].e[j], e[u].e[j], 0.0f);
+                    if constexpr (SUBTRACT) s[j] = score(k.l[u].e[j], k.e[u].e[j], f32(k.o[u].e[j]));
+                    else s[j] = score(k.l[u].e[j], k.e[u].e[j], 0.0f);
                 }
                 if (!SUBTRACT && static_cast<unsigned>(out - at) < 8u) {
 #pragma unroll
@@ -380,8 +394,17 @@ __device__ __forceinline__ void race(Best& best, const T* row, const Q* q, const
             }
         };
         int g = threadIdx.x;
-        for (; g + (OCTETS - 1) * THREADS < groups; g += OCTETS * THREADS) batch(g, std::true_type());
-        if (g < groups) batch(g, std::false_type());
+        if (g < groups) {
+            Octets k, then;
+            load(k, g);
+            while (g + OCTETS * THREADS < groups) {
+                load(then, g + OCTETS * THREADS);
+                use(k, g);
+                k = then;
+                g += OCTETS * THREADS;
+            }
+            use(k, g);
+        }
         v = lo + groups * 8;
     }
     for (v += threadIdx.x; v < hi; v += SINGLES * THREADS) {
