@@ -486,13 +486,16 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) adapt_few(AdaptParams p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Many rows an adapter (prefill): tiles of 64 rows, sixteen warps (four row groups by four shares of the columns), CTAS a
-// cluster. One ring of shared memory carries both products: stages of 64 k of x and A, then stages of 128 columns of y and
+// Many rows an adapter (prefill): tiles of 64 rows, CTAS a cluster; four shares of the columns by two groups of 32 rows
+// (eight warps of two fragments, two CTAs an SM) or, from rank 33 on, where shared memory leaves one CTA an SM, by four
+// groups of 16 (8192 x rank 16: 57 us against 64 with four groups; 3001 x rank 64: 73 against 76 with two). One ring of shared memory carries both products: stages of 64 k of x and A, then stages of 128 columns of y and
 // B, filled by 16-byte asynchronous copies, so that the second product's operands are on their way while the sums are
 // joined. Rows of a stage are 128 bytes or more apart and their 16-byte pieces swapped by halves on odd rows (piece ^ 4),
 // so that a quarter load (two rows, four pieces) meets every bank once.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int MANY_ROWS = 64, MANY_WARPS = 16, MANY_TILES = 6, MANY_COLS = MANY_TILES * 8 * 4;      // inner columns it holds
+constexpr int many_fragments(int rank16) { return rank16 >= 4 ? 1 : 2; }        // of 16 rows, a warp
+constexpr int many_warps(int rank16) { return 16 / many_fragments(rank16); }
+constexpr int MANY_ROWS = 64, MANY_TILES = 6, MANY_COLS = MANY_TILES * 8 * 4;      // inner columns it holds
 constexpr int stage_bytes(int cols, int rank16) {
     const int first = (MANY_ROWS + cols) * 128, second = MANY_ROWS * 256 + 128 * rank16 * 32;
     return first > second ? first : second;
@@ -503,12 +506,13 @@ constexpr int many_bytes(int cols, int rank16, int stages, int ctas) {
 }
 
 template <typename T, int RANK16, int CTAS>
-__global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_many(AdaptParams p, int stages) {
-    constexpr int M = MANY_ROWS, WARPS = MANY_WARPS, THREADS = WARPS * 32, RP = RANK16 * 16, OWN = SEGMENTS / CTAS;
+__global__ void __launch_bounds__(many_warps(RANK16) * 32, RANK16 >= 4 ? 1 : 2) adapt_many(AdaptParams p, int stages) {
+    constexpr int F = many_fragments(RANK16), GROUPS = 4 / F;
+    constexpr int M = MANY_ROWS, WARPS = many_warps(RANK16), THREADS = WARPS * 32, RP = RANK16 * 16, OWN = SEGMENTS / CTAS;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int tile_rows[M];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
-    const int row_warp = warp & 3, col_warp = warp >> 2;
+    const int row_warp = warp % GROUPS, col_warp = warp / GROUPS;
     const int rank = blockIdx.x % CTAS, tile = blockIdx.x / CTAS;
     const int cols = p.ad.n_mats * RP, slot_bytes = stage_bytes(cols, RANK16);
     const Inner<T> u(smem + stages * slot_bytes, M, cols);
@@ -533,24 +537,24 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
         n_first += (segment_at(k_blocks, rank * OWN + s + 1) - segment_at(k_blocks, rank * OWN + s) + 1) / 2;
     const int n_second = (block_hi - block_lo + 3) / 4, n_stages = n_first + n_second;
 
-    // What this thread copies of a first stage: piece tid % 8 of rows tid / 8 + 64 i of x (i = 0), then of A; of a second:
-    // piece tid % 16 of rows tid / 16 + 32 i of y, then of B's. Rows of x and y that the tile lacks are left as they are (no
-    // other row's result has anything of theirs).
+    // What this thread copies of a first stage: piece tid % 8 of rows tid / 8 + 32 i of x, then of A; of a second: piece tid
+    // % 16 of rows tid / 16 + 16 i of y, then of B's. Rows of x and y that the tile lacks are left as they are (no other
+    // row's result has anything of theirs).
     constexpr int TILES = RANK16 == 1 ? 2 : RANK16 == 2 ? 4 : MANY_TILES;       // n8 tiles of the first product a warp
-    constexpr int PIECES = 1 + (TILES * 8 * 4 + MANY_ROWS - 1) / MANY_ROWS, ROW = RANK16 * 2;   // ROW: pieces of a row of B
-    static_assert(MANY_ROWS * 8 == THREADS, "a piece of x a thread");
+    constexpr int STEP = THREADS / 8, X_PIECES = M / STEP, PIECES = X_PIECES + TILES * 8 * 4 / STEP;
+    constexpr int Y_STEP = THREADS / 16, Y_PIECES = M / Y_STEP, ROW = RANK16 * 2;       // ROW: pieces of a row of B
     const int piece = tid & 7, piece_row = tid >> 3;
     const T* from_first[PIECES];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-        const int a = piece_row + (i - 1) * MANY_ROWS;
-        if (i == 0) from_first[i] = tile_rows[piece_row] >= 0 ? x + tile_rows[piece_row] * p.x_stride + piece * 8 : nullptr;
+        const int r = piece_row + i * STEP, a = r - M;
+        if (i < X_PIECES) from_first[i] = tile_rows[r % M] >= 0 ? x + tile_rows[r % M] * p.x_stride + piece * 8 : nullptr;
         else from_first[i] = a < a_rows ? ad.a_row(a >> 3, a & 7) + piece * 8 : nullptr;
     }
-    const T* from_y[2];
+    const T* from_y[Y_PIECES];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int t = tile_rows[(tid >> 4) + i * 32];
+    for (int i = 0; i < Y_PIECES; ++i) {
+        const int t = tile_rows[(tid >> 4) + i * Y_STEP];
         from_y[i] = t >= 0 ? y + t * p.y_stride + (tid & 3) * 8 : nullptr;
     }
     const uint32_t ring = smem_addr(smem), ring_end = ring + stages * slot_bytes;
@@ -576,11 +580,11 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
             if (k + piece * 8 < min(fill_end * 32, K)) {
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i)
-                    if (from_first[i]) cp_async16_sa(to + i * MANY_ROWS * 128, from_first[i] + k);
+                    if (from_first[i]) cp_async16_sa(to + i * STEP * 128, from_first[i] + k);
             } else {
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i)
-                    if (i == 0 || from_first[i]) st_shared_zero(to + i * MANY_ROWS * 128);
+                    if (i < X_PIECES || from_first[i]) st_shared_zero(to + i * STEP * 128);
             }
             fill_block = min(fill_block + 2, fill_end);
         } else {
@@ -592,8 +596,8 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
             if (!all) block = b0 + by < block_hi ? block_at(p, b0 + by) : Block{0, 0, 0};
             if ((tid & 3) * 8 < block.left)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (from_y[i]) cp_async16_sa(fill_to + to_y + i * 32 * 256, from_y[i] + block.col);
+                for (int i = 0; i < Y_PIECES; ++i)
+                    if (from_y[i]) cp_async16_sa(fill_to + to_y + i * Y_STEP * 256, from_y[i] + block.col);
             // B: [block][j][g][RP]: row g of tile j is the block's column 8 (g / 2) + 2 j + g % 2
 #pragma unroll
             for (int i = 0; i < (128 * ROW + THREADS - 1) / THREADS; ++i) {
@@ -629,13 +633,13 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
     // u = x A^T, a segment at a time; sums of segments join as the tree's levels complete (level l of this thread's values
     // in shared memory, where u's halves will be).
     const int per = (ad.n_tiles + 3) / 4, t0 = col_warp * per, nt = min(per, ad.n_tiles - t0);
-    const int la = row_warp * 16 + g, lb = la + 8;
+    const int la = row_warp * 16 * F + g;       // the first of this lane's rows: la + 16 f and la + 16 f + 8
     float* levels = reinterpret_cast<float*>(u.hi);
     // lane (g, q)'s piece of half h of an even or odd row: q or q + 4
     const uint32_t x_at = la * 128 + q * 16, a_at = (M + t0 * 8 + g) * 128 + q * 16, odd = (g & 1) * 64;
 #pragma unroll
     for (int s = 0; s < OWN; ++s) {
-        float acc[TILES][4] = {};
+        float acc[F][TILES][4] = {};
         const int end = segment_at(k_blocks, rank * OWN + s + 1);
         for (int kb = segment_at(k_blocks, rank * OWN + s); kb < end; kb += 2) {
             const uint32_t from = next();
@@ -643,27 +647,37 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
             for (int h = 0; h < 2; ++h) {
                 if (kb + h >= end) break;
                 const uint32_t half = h * 64 ^ odd;
-                const uint4 va = ld_shared_v4(from + x_at + half), vb = ld_shared_v4(from + x_at + half + 8 * 128);
-                const uint32_t a0[4] = {va.x, vb.x, va.y, vb.y}, a1[4] = {va.z, vb.z, va.w, vb.w};
-                uint4 w[TILES];
+                uint4 v[F][2], w[TILES];
+#pragma unroll
+                for (int f = 0; f < F; ++f)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) v[f][r] = ld_shared_v4(from + x_at + half + (f * 16 + r * 8) * 128);
 #pragma unroll
                 for (int j = 0; j < TILES; ++j)
                     if (j < nt) w[j] = ld_shared_v4(from + a_at + half + j * 8 * 128);
 #pragma unroll
-                for (int j = 0; j < TILES; ++j)
-                    if (j < nt) mma<T>(acc[j], a0, w[j].x, w[j].y);
+                for (int f = 0; f < F; ++f) {
+                    const uint32_t a0[4] = {v[f][0].x, v[f][1].x, v[f][0].y, v[f][1].y};
+                    const uint32_t a1[4] = {v[f][0].z, v[f][1].z, v[f][0].w, v[f][1].w};
 #pragma unroll
-                for (int j = 0; j < TILES; ++j)
-                    if (j < nt) mma<T>(acc[j], a1, w[j].z, w[j].w);
+                    for (int j = 0; j < TILES; ++j)
+                        if (j < nt) mma<T>(acc[f][j], a0, w[j].x, w[j].y);
+#pragma unroll
+                    for (int j = 0; j < TILES; ++j)
+                        if (j < nt) mma<T>(acc[f][j], a1, w[j].z, w[j].w);
+                }
             }
         }
 #pragma unroll
-        for (int j = 0; j < TILES; ++j)
-            if (j < nt)
+        for (int j = 0; j < TILES; ++j) {
+            if (j >= nt) break;
+            const int col = ad.template column<RP>(t0 + j) + q * 2;
+#pragma unroll
+            for (int f = 0; f < F; ++f)
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
-                    const int at = (la + e * 4) * cols + ad.template column<RP>(t0 + j) + q * 2;
-                    float2 v = make_float2(acc[j][e], acc[j][e + 1]);
+                    const int at = (la + f * 16 + e * 4) * cols + col;
+                    float2 v = make_float2(acc[f][j][e], acc[f][j][e + 1]);
                     int level = 0;
 #pragma unroll
                     for (int bit = s; bit & 1; bit >>= 1, ++level) {
@@ -672,6 +686,7 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
                     }
                     *reinterpret_cast<float2*>(s == OWN - 1 ? &u.sums[at] : &levels[level * M * cols + at]) = v;
                 }
+        }
     }
     cluster_sync_all();
     const float scale = p.ad.scales ? p.ad.scales[mine.slot] : 1.0f;
@@ -679,13 +694,37 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
         join_row<T, RANK16, CTAS>(u, r, ad.r8, scale);
     cluster_sync_all();     // (the last access to another CTA's memory was before it)
 
-    const int ra = tile_rows[la], rb = tile_rows[lb];
-    const float fa = u.factor[la], fb = u.factor[lb];
-    T* out_a = ra >= 0 ? static_cast<T*>(p.out) + ra * p.out_stride + q * 8 : nullptr;
-    T* out_b = rb >= 0 ? static_cast<T*>(p.out) + rb * p.out_stride + q * 8 : nullptr;
+    T* to[F][2];
+    float scale_of[F][2];
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = la + f * 16 + r * 8, at = tile_rows[row];
+            to[f][r] = at >= 0 ? static_cast<T*>(p.out) + at * p.out_stride + q * 8 : nullptr;
+            scale_of[f][r] = u.factor[row];
+        }
     const uint32_t y_at = la * 256 + (col_warp * 4 + q ^ (g & 1) << 2) * 16;
     const uint32_t b_at = M * 256 + (col_warp * 32 + g) * ROW * 16;
-    const uint32_t u_at = smem_addr(u.hi + la * u.stride), lo_off = M * u.stride * sizeof(T), down = 8 * u.stride * sizeof(T);
+    const uint32_t row_bytes = u.stride * sizeof(T), u_at = smem_addr(u.hi) + la * row_bytes, lo_off = M * row_bytes;
+    // hi and lo of steps s and s + 1 of row fragment f, for the matrix whose halves start at `at`
+    const auto fragments = [&](uint32_t at, int f, int s, uint32_t (&hi)[2][4], uint32_t (&lo)[2][4]) {
+        const uint32_t a = at + f * 16 * row_bytes, b = a + 8 * row_bytes;
+        if constexpr (RANK16 == 1) {
+            const uint2 h0 = ld_shared_v2(a + q * 8), h1 = ld_shared_v2(b + q * 8);
+            const uint2 l0 = ld_shared_v2(a + lo_off + q * 8), l1 = ld_shared_v2(b + lo_off + q * 8);
+            hi[0][0] = h0.x, hi[0][1] = h1.x, hi[0][2] = h0.y, hi[0][3] = h1.y;
+            lo[0][0] = l0.x, lo[0][1] = l1.x, lo[0][2] = l0.y, lo[0][3] = l1.y;
+        } else {
+            const uint32_t off = s * 32 + q * 16;
+            const uint4 h0 = ld_shared_v4(a + off), h1 = ld_shared_v4(b + off);
+            const uint4 l0 = ld_shared_v4(a + lo_off + off), l1 = ld_shared_v4(b + lo_off + off);
+            hi[0][0] = h0.x, hi[0][1] = h1.x, hi[0][2] = h0.y, hi[0][3] = h1.y;
+            hi[1][0] = h0.z, hi[1][1] = h1.z, hi[1][2] = h0.w, hi[1][3] = h1.w;
+            lo[0][0] = l0.x, lo[0][1] = l1.x, lo[0][2] = l0.y, lo[0][3] = l1.y;
+            lo[1][0] = l0.z, lo[1][1] = l1.z, lo[1][2] = l0.w, lo[1][3] = l1.w;
+        }
+    };
     for (int i = 0; i < n_second; ++i) {
         const uint32_t from = next();
         const int b0 = block_lo + i * 4;
@@ -694,44 +733,45 @@ __global__ void __launch_bounds__(MANY_WARPS * 32, RANK16 >= 4 ? 1 : 2) adapt_ma
         advance(use_at, b0 + 4);
         if (block.left <= 0) continue;
         const uint32_t u_m = u_at + block.m * RP * sizeof(T);
-        float acc[4][4] = {};
-        if constexpr (RANK16 == 1) {
-            const uint2 h0 = ld_shared_v2(u_m + q * 8), h1 = ld_shared_v2(u_m + down + q * 8);
-            const uint2 l0 = ld_shared_v2(u_m + lo_off + q * 8), l1 = ld_shared_v2(u_m + lo_off + down + q * 8);
-            const uint32_t hi[4] = {h0.x, h1.x, h0.y, h1.y}, lo[4] = {l0.x, l1.x, l0.y, l1.y};
-            uint2 w[4];
+        float acc[F][4][4] = {};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = ld_shared_v2(from + b_at + j * 8 * ROW * 16 + q * 8);
+        for (int s = 0; s < RANK16; s += 2) {
+            if (s * 16 >= ad.r8) break;
+            uint4 w[4];
+            const uint32_t c = RANK16 >= 4 ? (s * 2 + q ^ (g & 1) << 2) * 16 : q * 16;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma<T>(acc[j], hi, w[j].x, w[j].y);
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (RANK16 == 1) {
+                    const uint2 v = ld_shared_v2(from + b_at + j * 8 * ROW * 16 + q * 8);
+                    w[j] = {v.x, v.y, 0, 0};
+                } else {
+                    w[j] = ld_shared_v4(from + b_at + j * 8 * ROW * 16 + c);
+                }
+            }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma<T>(acc[j], lo, w[j].x, w[j].y);
-        } else {
+            for (int f = 0; f < F; ++f) {
+                uint32_t hi[2][4], lo[2][4];
+                fragments(u_m, f, s, hi, lo);
 #pragma unroll
-            for (int s = 0; s < RANK16; s += 2) {
-                if (s * 16 >= ad.r8) break;
-                const uint4 h0 = ld_shared_v4(u_m + s * 32 + q * 16), h1 = ld_shared_v4(u_m + down + s * 32 + q * 16);
-                const uint4 l0 = ld_shared_v4(u_m + lo_off + s * 32 + q * 16);
-                const uint4 l1 = ld_shared_v4(u_m + lo_off + down + s * 32 + q * 16);
-                const uint32_t h_a[4] = {h0.x, h1.x, h0.y, h1.y}, h_b[4] = {h0.z, h1.z, h0.w, h1.w};
-                const uint32_t l_a[4] = {l0.x, l1.x, l0.y, l1.y}, l_b[4] = {l0.z, l1.z, l0.w, l1.w};
-                const uint32_t c = RANK16 >= 4 ? (s * 2 + q ^ (g & 1) << 2) * 16 : q * 16;
-                uint4 w[4];
+                for (int j = 0; j < 4; ++j) mma<T>(acc[f][j], hi[0], w[j].x, w[j].y);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = ld_shared_v4(from + b_at + j * 8 * ROW * 16 + c);
+                for (int j = 0; j < 4; ++j) mma<T>(acc[f][j], lo[0], w[j].x, w[j].y);
+                if constexpr (RANK16 > 1) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mma<T>(acc[j], h_a, w[j].x, w[j].y);
+                    for (int j = 0; j < 4; ++j) mma<T>(acc[f][j], hi[1], w[j].z, w[j].w);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mma<T>(acc[j], l_a, w[j].x, w[j].y);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mma<T>(acc[j], h_b, w[j].z, w[j].w);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mma<T>(acc[j], l_b, w[j].z, w[j].w);
+                    for (int j = 0; j < 4; ++j) mma<T>(acc[f][j], lo[1], w[j].z, w[j].w);
+                }
             }
         }
         if (q * 8 >= block.left) continue;
-        if (out_a) *reinterpret_cast<uint4*>(out_a + block.col) = added<T>(ld_shared_v4(from + y_at), acc, 0, fa);
-        if (out_b) *reinterpret_cast<uint4*>(out_b + block.col) = added<T>(ld_shared_v4(from + y_at + 8 * 256), acc, 2, fb);
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                if (to[f][r])
+                    *reinterpret_cast<uint4*>(to[f][r] + block.col) =
+                        added<T>(ld_shared_v4(from + y_at + (f * 16 + r * 8) * 256), acc[f], r * 2, scale_of[f][r]);
     }
     cp_async_wait<0>();
 }
@@ -837,7 +877,7 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
     const size_t smem = many_bytes(cols, steps, stages, ctas);
     const auto kernel = half ? many_kernel<__half>(steps, ctas) : many_kernel<__nv_bfloat16>(steps, ctas);
     if (const int rc = allow_smem(kernel, std::max<size_t>(smem, 49153))) return rc;
-    if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * ctas), dim3(MANY_WARPS * 32), smem,
+    if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * ctas), dim3(many_warps(steps) * 32), smem,
                                       stream, true, ctas, p, stages))
         return rc;
     return ok();
