@@ -6,9 +6,9 @@
 // Bytes bound it where there are many requests (a row of 248320 bf16 logits is 0.5 MB, a request's noise 1 MB): rows past
 // the first that falls are never read. With few, latency does: rows are taken one after another, about 2.5 us each (one
 // pass over the row, one exchange in the cluster), then the race, 2.9 us. Measured: one request of 3 drafted tokens 11 us,
-// 13 ragged ones (fp32, 150001 ids) 19 us, 96 requests 74 us for the 210 MB they cannot do without (44% of a plain copy;
-// the exponentials alone take the special-function units 28% of that time, the rest is waits at the rows' ends, which more
-// and smaller CTAs only trade for more of them).
+// 13 ragged ones (fp32, 150001 ids) 19 us, 96 requests 70 us for the 210 MB they cannot do without (47% of a plain copy;
+// the exponentials alone take the special-function units about 30% of that time, the rest is waits at the rows' ends, which
+// more and smaller CTAs only trade for more of them).
 #include <cuda_runtime.h>
 
 #include <limits.h>
@@ -494,7 +494,6 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) verify_kernel(VerifyParams 
             fence_mbar_init();
             exchange.arm(r);
         }
-        prefetch_l2(noise + lo, static_cast<size_t>(hi - lo) * sizeof(float));
     }
     pdl_launch_dependents();
     pdl_wait();
@@ -549,6 +548,10 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) verify_kernel(VerifyParams 
         if (!greedy) {
             const float mc = m * c;
             const Weights wt{m, c, mc, safe ? inv_z : inv_z * ex2(-fmaf(m, c, -mc))};
+            // On its way while the race's first loads are: 96 requests 70 us, 71 with no such order. Given at the start of
+            // the kernel instead it takes 75: a fifth of these requests are greedy and never read their noise, and the
+            // others' (a MB each) displaces rows that the race reads again.
+            if (threadIdx.x == 0) prefetch_l2(noise + lo, static_cast<size_t>(hi - lo) * sizeof(float));
             const int out = GIVEN ? -1 : d;
             if (GIVEN && i < k) {
                 if constexpr (GIVEN) {
