@@ -292,3 +292,51 @@ def test_library_refusals():
         assert call(t=1000) == _lib.ESP_ERR_SCRATCH
         assert call(t=1000, ws=16, ws_bytes=lib.esp_adapt_ws_bytes(1000, 2) - 1) == _lib.ESP_ERR_SCRATCH
         assert call(t=1000, ws=20, ws_bytes=1 << 20) == _lib.ESP_ERR_SCRATCH
+
+
+# Tiles of 64 rows (more than 1024 rows on 148 SMs, 24 or 40 an adapter): the same properties there.
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank", [8, 16, 24, 32, 40, 56, 64, 72, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("widths", [[264], [256, 72], [256, 72, 40]])
+def test_prefill_ranks(dev, rank, dtype, widths):
+    ad = make(dev, dtype, 528, widths, 7, rank, rank)
+    x, y, i = rows(dev, ad, 1100, rank, "runs" if rank % 16 else "mixed")
+    check(ad(x, y, i), ad, x, y, i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [8, 24, 40, 256, 1032, 6000])
+@pytest.mark.parametrize("widths", [[8], [40], [136, 8, 24], [256, 256, 64, 32], [1400, 136, 136]])
+@pytest.mark.parametrize("rank", [16, 32])
+def test_prefill_shapes(dev, k, widths, rank):
+    ad = make(dev, torch.float16 if k % 16 else torch.bfloat16, k, widths, 3, rank, k)
+    x, y, i = rows(dev, ad, 1090, k)
+    check(ad(x, y, i), ad, x, y, i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1024, 1025, 1039, 1087, 1088, 1089, 4100])
+@pytest.mark.parametrize("slots,ids", [(5, "runs"), (5, "mixed"), (42, "runs"), (46, "mixed")])
+def test_prefill_batches(dev, T, slots, ids):
+    ad = make(dev, torch.bfloat16, 256, [128, 40, 40], slots, 32, T)
+    x, y, i = rows(dev, ad, T, T, ids)
+    check(ad(x, y, i), ad, x, y, i)
+
+
+@pytest.mark.gpu
+def test_prefill_rows_streams_and_strides(dev):
+    test_no_ranks_no_scales(dev, 1200)
+    test_rows_without_an_adapter_keep_y(dev, 1201)
+    test_strides_and_in_place(dev, 1202)
+    test_streams_and_graphs(dev, 1203)
+
+
+@pytest.mark.gpu
+def test_a_rows_bits_are_its_own_at_rank_32(dev):
+    """Rank 32 of three matrices takes shorter rings in a prefill: the same bits as in a decode batch and alone."""
+    ad = make(dev, torch.bfloat16, 2048, [1024, 256, 256], 4, 32, 3)
+    x, y, i = rows(dev, ad, 2000, 1)
+    want = ad(x, y, i)
+    for lo, hi in ((0, 1), (5, 45), (100, 300), (0, 1024), (0, 1025)):
+        assert torch.equal(ad(x[lo:hi], y[lo:hi], i[lo:hi].contiguous()), want[lo:hi])

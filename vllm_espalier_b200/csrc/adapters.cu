@@ -30,7 +30,9 @@ namespace esp {
 namespace {
 
 constexpr int SEGMENTS = 8, MAX_SLOTS = 4096;
-constexpr int NO_PLAN = 64;             // up to this many rows every CTA finds its tile's rows itself
+// Up to this many rows every CTA finds its tile's rows itself, above it a launch of its own does: 17 / 32 / 48 / 64 rows 7.6 /
+// 8.2 / 9.0 / 10.7 us so, 10.1 / 11.1 / 10.9 / 11.1 with the plan.
+constexpr int NO_PLAN = 64;
 
 struct AdaptParams {
     esp_adapters_t ad;
@@ -495,10 +497,11 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) adapt_few(AdaptParams p) {
 // ---------------------------------------------------------------------------------------------------------------
 // Many rows an adapter (prefill): tiles of 64 rows, CTAS a cluster; four shares of the columns by two groups of 32 rows
 // (eight warps of two fragments, two CTAs an SM) or, from rank 33 on, where shared memory leaves one CTA an SM, by four
-// groups of 16 (8192 x rank 16: 57 us against 64 with four groups; 3001 x rank 64: 73 against 76 with two). One ring of shared memory carries both products: stages of 64 k of x and A, then stages of 128 columns of y and
-// B, filled by 16-byte asynchronous copies, so that the second product's operands are on their way while the sums are
-// joined. Rows of a stage are 128 bytes or more apart and their 16-byte pieces swapped by halves on odd rows (piece ^ 4),
-// so that a quarter load (two rows, four pieces) meets every bank once.
+// groups of 16 (8192 x rank 16: 57 us against 64 with four groups; x rank 32: 97 against 95, but 69 against 80 with one
+// matrix; 3001 x rank 64: 73 against 76 with two). One ring of shared memory carries both products: stages of 64 k of x and
+// A, then stages of 128 columns of y and B, filled by 16-byte asynchronous copies, so that the second product's operands are
+// on their way while the sums are joined. Rows of a stage are 128 bytes or more apart and their 16-byte pieces swapped by
+// halves on odd rows (piece ^ 4), so that a quarter load (two rows, four pieces) meets every bank once.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int many_fragments(int rank16) { return rank16 >= 4 ? 1 : 2; }        // of 16 rows, a warp
 constexpr int many_warps(int rank16) { return 16 / many_fragments(rank16); }
@@ -628,7 +631,8 @@ __global__ void __launch_bounds__(many_warps(RANK16) * 32, RANK16 >= 4 ? 1 : 2) 
     uint32_t use = ring;
     const auto next = [&] {         // the next stage, whole and for all; the one behind it is filled again
         if (stages == 4) cp_async_wait<2>();
-        else cp_async_wait<1>();
+        else if (RANK16 != 2 || stages == 3) cp_async_wait<1>();
+        else cp_async_wait<0>();
         __syncthreads();
         fill();
         cp_async_commit();
@@ -846,8 +850,12 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
 
     const int steps = rank_steps(ad->rank), cols = ad->n_mats * steps * 16;
     const bool half = ad->dtype == F16;
-    // Tiles of 64 rows where adapters have half of that on average and their inner columns fit a CTA.
-    const bool many = t_rows > NO_PLAN && t_rows / ad->slots >= 32 && cols <= MANY_COLS;
+    // Tiles of 64 rows where the inner columns fit a CTA, tiles of 16 need more than two rounds of the GPU's clusters, and
+    // adapters have enough rows each that tiles of 64 are not mostly empty. Measured, 16 / 64 rows a tile, us, rank 16, 32 and
+    // 64: 512 rows 15 / 17, 18 / 23, 22 / 24; 1024 rows 21 / 20, 26 / 27, 34 / 39; 1536 rows 30 / 21, 37 / 28, 49 / 39. 64
+    // adapters mixed row by row: 1536 rows 41 / 32, 51 / 47, 67 / 100; 3000 rows 66 / 37, 80 / 55, 102 / 104.
+    const int clusters = std::max(device_sms() / 18, 1) * (18 * 2 / FEW_CTAS);
+    const bool many = t_rows > 2 * FEW_ROWS * clusters && t_rows / ad->slots >= (steps >= 4 ? 40 : 24) && cols <= MANY_COLS;
     const int m = many ? MANY_ROWS : FEW_ROWS;
     AdaptParams p{*ad, x, y, ids, out, nullptr, x_stride, y_stride, out_stride, t_rows, static_cast<int>(n), t_rows};
     if (t_rows > NO_PLAN) {
@@ -868,19 +876,24 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
         return ok();
     }
     // CTAs a tile: what takes the least rounds x (a CTA's share of a tile + what it spends on joining sums). Places: two CTAs
-    // an SM (one from rank 33 on), as many whole clusters as the 18 SMs of a GPC hold. Measured: 128 tiles of rank 16 with 2 /
-    // 4 / 8 CTAs 68 / 74 / 90 us, 47 tiles of rank 64 with 4 / 8 75 / 85 us.
-    const int an_sm = steps >= 4 ? 1 : 2, tiles = (t_rows + m - 1) / m + std::min(ad->slots, t_rows / m) / 2;
+    // an SM (one from rank 33 on, or where a ring of two stages does not fit twice), as many whole clusters as the 18 SMs of a
+    // GPC hold. Measured: 128 tiles of rank 16 with 2 / 4 / 8 CTAs 68 / 74 / 90 us, 47 tiles of rank 64 with 4 / 8 75 / 85 us.
+    const int half_sm = MAX_SMEM / 2 - 1024, tiles = (t_rows + m - 1) / m + std::min(ad->slots, t_rows / m) / 2;
     int ctas = 8;       // (fits whatever fits at all)
     double best = 1e30;
     for (int c : {2, 4, 8}) {
         if (many_bytes(cols, steps, 3, c) > MAX_SMEM) continue;
+        const int an_sm = steps < 4 && many_bytes(cols, steps, steps == 2 ? 2 : 3, c) <= half_sm ? 2 : 1;
         const int places = std::max(device_sms() / 18, 1) * (18 * an_sm / c) * c;
         const double work = ((tiles * c + places - 1) / places) * (1.0 / c + CTA_COST);
         if (work < best) best = work, ctas = c;
     }
-    const int room = steps >= 4 ? MAX_SMEM : MAX_SMEM / 2 - 1024;
-    const int stages = many_bytes(cols, steps, 4, ctas) <= room ? 4 : 3;
+    // Two stages where that leaves an SM to two CTAs: q | k | v at rank 32, 8192 rows 97 us against 125 with three and one CTA.
+    const bool three = steps != 2 || many_bytes(cols, steps, 3, ctas) <= half_sm;
+    const int least = three || many_bytes(cols, steps, 2, ctas) > half_sm ? 3 : 2;
+    const int room = steps < 4 && many_bytes(cols, steps, least, ctas) <= half_sm ? half_sm : MAX_SMEM;
+    int stages = 4;
+    while (stages > least && many_bytes(cols, steps, stages, ctas) > room) --stages;
     const size_t smem = many_bytes(cols, steps, stages, ctas);
     const auto kernel = half ? many_kernel<__half>(steps, ctas) : many_kernel<__nv_bfloat16>(steps, ctas);
     if (const int rc = allow_smem(kernel, std::max<size_t>(smem, 49153))) return rc;
