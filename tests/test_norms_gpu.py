@@ -9,6 +9,11 @@ of s itself, E' = E rms(M) / s. Rounding is monotone, so an output lies between 
 """
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -307,3 +312,16 @@ def test_library_refusals():
         assert call(op=other) == _lib.ESP_ERR_INVALID, name
     with pytest.raises(EspError):
         _lib.check(call(rows=-1))
+
+
+@pytest.mark.gpu
+def test_widths_around_the_default_shared_memory():
+    """Rows of about 48 KB of fp32 in a process of its own: a wider row before them would have raised the kernel's limit."""
+    code = ("import torch, test_norms_gpu as t\n"
+            "for d in (12288, 12257, 12256, 8193, 12289):\n"
+            "    t.run_and_check(torch.device('cuda:0'), 3, d, torch.bfloat16, torch.float32, 'layer', two=True, "
+            "gate='channel', act='tanh', seed=d)\n")
+    here = Path(__file__).resolve().parent
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(here.parent), str(here), os.environ.get("PYTHONPATH", "")]))
+    done = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=600)
+    assert done.returncode == 0, done.stderr[-2000:]

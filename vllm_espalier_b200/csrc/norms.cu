@@ -672,8 +672,9 @@ extern "C" int esp_block_norm(const esp_block_norm_op_t* op, const void* x, long
         if (const int rc = launch(k.run, dim3(static_cast<unsigned>(rows)), dim3(k.threads), 0, stream, true, p)) return rc;
         return ok();
     }
+    // (49153: 48 KB are what a CTA has without asking, its static words among them, so rows of just under that ask as well)
     const size_t smem = static_cast<size_t>(op->d) * 4;
-    if (const int rc = allow_smem(block_norm_kernel, smem)) return rc;
+    if (const int rc = allow_smem(block_norm_kernel, std::max<size_t>(smem, 49153))) return rc;
     if (const int rc = launch(block_norm_kernel, dim3(static_cast<unsigned>(rows)), dim3(op->d <= 4096 ? 256 : 1024), smem,
                               stream, true, p))
         return rc;
