@@ -8,6 +8,8 @@ fp32 rounding. Rounding to the output's type is monotone, so an output lies betw
 """
 from __future__ import annotations
 
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
@@ -340,3 +342,32 @@ def test_a_rows_bits_are_its_own_at_rank_32(dev):
     want = ad(x, y, i)
     for lo, hi in ((0, 1), (5, 45), (100, 300), (0, 1024), (0, 1025)):
         assert torch.equal(ad(x[lo:hi], y[lo:hi], i[lo:hi].contiguous()), want[lo:hi])
+
+
+@pytest.mark.gpu
+def test_threads_of_different_adapters(dev):
+    """Host threads on streams of their own use adapters of one rank and of one matrix or three: one kernel, two amounts of
+    shared memory."""
+    calls = []
+    for widths in ([128], [128, 64, 64]):
+        ad = make(dev, torch.bfloat16, 256, widths, 3, 64, 7)
+        calls += [(ad, rows(dev, ad, 1100, 5))] * 2
+    want = [ad(*r) for ad, r in calls]
+
+    def work(call):
+        (ad, (x, y, ids)), stream = call, torch.cuda.Stream()
+        out, need = torch.empty_like(y), _lib.lib().esp_adapt_ws_bytes(1100, 3)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        at = (ad._ref, x.data_ptr(), ad.k, y.data_ptr(), ad.n, ids.data_ptr(), 1100, out.data_ptr(), ad.n, ws.data_ptr(), need,
+              stream.cuda_stream)
+        refused = 0
+        for i in range(2000):
+            refused += _lib.lib().esp_adapt(*at) != _lib.ESP_OK
+            if i % 50 == 49:
+                stream.synchronize()
+        stream.synchronize()
+        return refused, out
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(4) as pool:
+        for (refused, out), expected in zip(pool.map(work, calls), want):
+            assert refused == 0 and torch.equal(out, expected)

@@ -12,6 +12,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 import pytest
@@ -325,3 +326,32 @@ def test_widths_around_the_default_shared_memory():
     env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(here.parent), str(here), os.environ.get("PYTHONPATH", "")]))
     done = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=600)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_threads_of_different_widths(dev):
+    """Host threads on streams of their own launch one kernel with different amounts of shared memory: the wide rows' kernel
+    at two widths, the rows' ring with and without a second input."""
+    g = torch.Generator(device=dev).manual_seed(1)
+    wide, ring = [norms.BlockNorm(d, pre=True) for d in (13000, 40000)], norms.BlockNorm(4096, pre=True)
+    w = [torch.randn(1, op.d, device=dev, generator=g) for op in wide]
+    x = torch.randn(400, 4096, device=dev, generator=g).to(torch.bfloat16)
+    calls = [(op, t, None) for op, t in zip(wide, w)] + [(ring, x, None), (ring, x, x)]
+    want = [op(t, x2=x2)[1] for op, t, x2 in calls]
+
+    def work(call):
+        (op, t, x2), stream = call, torch.cuda.Stream()
+        r, h = torch.empty_like(t), torch.empty_like(t)
+        code = 2 if t.dtype == torch.float32 else 1
+        at = (op._ref, t.data_ptr(), op.d, x2.data_ptr() if x2 is not None else None, op.d, code, None, 0, code, None, 0, 0, 0,
+              r.data_ptr(), op.d, h.data_ptr(), op.d, t.shape[0], stream.cuda_stream)
+        refused = 0
+        for i in range(3000):
+            refused += _lib.lib().esp_block_norm(*at) != _lib.ESP_OK
+            if i % 100 == 99:
+                stream.synchronize()
+        return refused, h
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(4) as pool:
+        for (refused, h), expected in zip(pool.map(work, calls), want):
+            assert refused == 0 and torch.equal(h, expected)

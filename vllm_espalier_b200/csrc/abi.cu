@@ -55,6 +55,34 @@ int device_sms() {
     return cache[dev];
 }
 
+int allow_any_smem(const void* kernel, size_t bytes) {
+    if (bytes <= 47 * 1024) return ESP_OK;      // (48 KB without asking, a kernel's static words among them)
+    struct Asked {
+        const void* kernel;
+        int dev;
+    };
+    constexpr int MOST = 1024;                  // above the library's kernels x a machine's GPUs; past it each call asks
+    static std::mutex mutex;
+    static Asked asked[MOST];
+    static int n = 0;
+    int dev = 0, most = 0;
+    cudaFuncAttributes attr;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) {
+        const std::lock_guard<std::mutex> lock(mutex);
+        for (int i = 0; i < n; ++i)
+            if (asked[i].kernel == kernel && asked[i].dev == dev) return ESP_OK;
+        e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, kernel);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     most - static_cast<int>(attr.sharedSizeBytes));
+        if (e == cudaSuccess && n < MOST) asked[n++] = {kernel, dev};
+    }
+    if (e != cudaSuccess) return set_error(ESP_ERR_CUDA, "shared memory opt-in (%zu B): %s", bytes, cudaGetErrorString(e));
+    return ESP_OK;
+}
+
 }  // namespace esp
 
 extern "C" {

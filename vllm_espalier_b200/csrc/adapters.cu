@@ -869,7 +869,7 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
     if (!many) {
         const auto kernel = half ? few_kernel<__half>(steps) : few_kernel<__nv_bfloat16>(steps);
         const size_t smem = sums_bytes(m, cols) + halves_bytes(m, cols);
-        if (const int rc = allow_smem(kernel, std::max<size_t>(smem, 49153))) return rc;
+        if (const int rc = allow_any_smem(kernel, smem)) return rc;
         if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * FEW_CTAS), dim3(FEW_WARPS * 32),
                                           smem, stream, true, FEW_CTAS, p))
             return rc;
@@ -896,7 +896,7 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
     while (stages > least && many_bytes(cols, steps, stages, ctas) > room) --stages;
     const size_t smem = many_bytes(cols, steps, stages, ctas);
     const auto kernel = half ? many_kernel<__half>(steps, ctas) : many_kernel<__nv_bfloat16>(steps, ctas);
-    if (const int rc = allow_smem(kernel, std::max<size_t>(smem, 49153))) return rc;
+    if (const int rc = allow_any_smem(kernel, smem)) return rc;
     if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * ctas), dim3(many_warps(steps) * 32), smem,
                                       stream, true, ctas, p, stages))
         return rc;

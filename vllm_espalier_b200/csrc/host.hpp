@@ -83,6 +83,14 @@ int allow_smem(K kernel, size_t bytes) {
     return ESP_OK;
 }
 
+// For a kernel whose calls need different amounts of dynamic shared memory, before a launch with `bytes`: once per kernel
+// and device its limit becomes what the device has, so no call lowers it under another host thread's.
+int allow_any_smem(const void* kernel, size_t bytes);
+template <typename... KArgs>
+int allow_any_smem(void (*kernel)(KArgs...), size_t bytes) {
+    return allow_any_smem(reinterpret_cast<const void*>(kernel), bytes);
+}
+
 // Opt a kernel into clusters of more than eight CTAs.
 template <typename K>
 int allow_cluster16(K kernel) {

@@ -663,7 +663,7 @@ extern "C" int esp_block_norm(const esp_block_norm_op_t* op, const void* x, long
         // 1184 5.9 / 5.9, 8192 34 / 37; 4096 wide with a fp32 stream: 148 rows 4.3 / 3.4 us, 1200 15.4 / 16.7, 4096 41 / 52.
         if (rows > static_cast<long long>(k.ctas) * device_sms() && stages >= 2) {
             const int smem = stages * row_bytes(p);
-            if (const int rc = allow_smem(k.ring, std::max(smem, 49153))) return rc;
+            if (const int rc = allow_any_smem(k.ring, smem)) return rc;
             if (const int rc = launch(k.ring, dim3(k.ctas * device_sms()), dim3(k.threads), smem, stream, true, p,
                                       static_cast<int>(rows), stages))
                 return rc;
@@ -672,9 +672,8 @@ extern "C" int esp_block_norm(const esp_block_norm_op_t* op, const void* x, long
         if (const int rc = launch(k.run, dim3(static_cast<unsigned>(rows)), dim3(k.threads), 0, stream, true, p)) return rc;
         return ok();
     }
-    // (49153: 48 KB are what a CTA has without asking, its static words among them, so rows of just under that ask as well)
     const size_t smem = static_cast<size_t>(op->d) * 4;
-    if (const int rc = allow_smem(block_norm_kernel, std::max<size_t>(smem, 49153))) return rc;
+    if (const int rc = allow_any_smem(block_norm_kernel, smem)) return rc;
     if (const int rc = launch(block_norm_kernel, dim3(static_cast<unsigned>(rows)), dim3(op->d <= 4096 ? 256 : 1024), smem,
                               stream, true, p))
         return rc;
