@@ -17,6 +17,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from vllm_espalier_b200 import EspError, norms
 from vllm_espalier_b200 import _lib
@@ -355,3 +356,15 @@ def test_threads_of_different_widths(dev):
     with ThreadPoolExecutor(4) as pool:
         for (refused, h), expected in zip(pool.map(work, calls), want):
             assert refused == 0 and torch.equal(h, expected)
+
+
+def test_weights_on_another_device_are_refused():
+    """No GPU needed: tensors without storage, refused before anything reads them."""
+    with FakeTensorMode():
+        w = [torch.empty(64, device=f"cuda:{i}") for i in (0, 1)]
+        for kw in (dict(pre=w[0], post=w[1]), dict(pre=w[0], pre_bias=w[1])):
+            with pytest.raises(ValueError, match="device"):
+                norms.BlockNorm(64, **kw)
+        for kw in (dict(pre=w[1]), dict(post=w[1], pre=True), dict(pre=w[1], pre_bias=w[1])):
+            with pytest.raises(ValueError, match="device|cuda:1"):
+                norms.BlockNorm(64, **kw)(torch.empty(2, 64, device="cuda:0"))

@@ -50,9 +50,11 @@ class BlockNorm:
                     if not t.is_cuda or t.shape != (d,) or t.dtype not in DTYPE:
                         raise ValueError(f"{name} weight and bias must be CUDA fp16/bf16/fp32 [{d}] tensors")
                     tensors[key] = t.contiguous()
-        dtypes = {t.dtype for t in tensors.values()}
-        if len(dtypes) > 1:
-            raise ValueError(f"the weights and biases of one BlockNorm share a dtype, got {sorted(map(str, dtypes))}")
+        dtypes, devices = {t.dtype for t in tensors.values()}, {t.device for t in tensors.values()}
+        if len(dtypes) > 1 or len(devices) > 1:
+            raise ValueError(f"the weights and biases of one BlockNorm share a dtype and a device, got "
+                             f"{sorted(map(str, dtypes))} on {sorted(map(str, devices))}")
+        self.device = devices.pop() if devices else None        # of the weights; none without any
         self.d, self.kind, self.has_pre, self.tensors = d, kind, on["pre"], tensors
         at = {k: t.data_ptr() for k, t in tensors.items()}
         self._op = esp_block_norm_op_t(d, KINDS[kind] * on["post"], KINDS[kind] * on["pre"], ACTS[gate_act], eps,
@@ -77,6 +79,8 @@ class BlockNorm:
         x_code = DTYPE.get(x_dtype)
         if x.dim() != 2 or x.shape[1] != d or not x.is_cuda or x_code is None:
             raise ValueError(f"x must be a CUDA fp16/bf16/fp32 [rows, {d}] tensor, got {x_dtype} {tuple(x.shape)}")
+        if self.device is not None and x.device != self.device:
+            raise ValueError(f"x must be on the weights' {self.device}, got {x.device}")
         x_stride, step = x.stride()
         if step != 1:
             x = x.contiguous()
