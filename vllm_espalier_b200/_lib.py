@@ -120,6 +120,17 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def launch(device: torch.device, entry, *args):
+    """entry(*args, stream) on the device's current stream, with the device current: a launch, a kernel's limits and the
+    default stream's handle are the current device's, and the arguments' need not be that one."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        check(entry(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(entry(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

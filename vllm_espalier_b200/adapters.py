@@ -14,7 +14,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import DTYPE, check, esp_adapters_t, lib, stream_ptr
+from ._lib import DTYPE, esp_adapters_t, launch, lib
 
 MAX_RANK, MAX_MATS, MAX_SLOTS = 128, 4, 4096
 NONE = -1                     # the id of a row without an adapter
@@ -142,8 +142,8 @@ class Adapters:
             need = lib().esp_adapt_ws_bytes(rows, self.slots)
             scratch = ids.new_empty((need + 3) // 4)
             ws = scratch.data_ptr()
-        check(lib().esp_adapt(self._ref, x.data_ptr(), x_stride, y.data_ptr(), y_stride, ids.data_ptr(), rows,
-                              out.data_ptr(), out_stride, ws, need, stream_ptr(self.device)))
+        launch(self.device, lib().esp_adapt, self._ref, x.data_ptr(), x_stride, y.data_ptr(), y_stride, ids.data_ptr(), rows,
+               out.data_ptr(), out_stride, ws, need)
         return out
 
     __call__ = forward

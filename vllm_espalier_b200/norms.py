@@ -16,7 +16,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import DTYPE, check, esp_block_norm_op_t, lib, stream_ptr
+from ._lib import DTYPE, esp_block_norm_op_t, launch, lib
 
 KINDS = {"rms": 1, "layer": 2}
 ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
@@ -124,9 +124,9 @@ class BlockNorm:
         elif normed is not None:
             raise ValueError("normed given, but this BlockNorm has no pre norm")
         if rows:
-            check(lib().esp_block_norm(self._ref, x.data_ptr(), x_stride, x2_ptr, x2_stride, x_code, residual_ptr,
-                                       residual_stride, r_code, gate_ptr, kind, gate_dtype, gate_stride,
-                                       out.data_ptr(), r_stride, h_ptr, h_stride, rows, stream_ptr(x.device)))
+            launch(x.device, lib().esp_block_norm, self._ref, x.data_ptr(), x_stride, x2_ptr, x2_stride, x_code,
+                   residual_ptr, residual_stride, r_code, gate_ptr, kind, gate_dtype, gate_stride, out.data_ptr(), r_stride,
+                   h_ptr, h_stride, rows)
         return out, normed
 
     @staticmethod

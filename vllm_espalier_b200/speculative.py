@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import DTYPE, check, lib, stream_ptr
+from ._lib import DTYPE, launch, lib
 
 
 def verify(logits: torch.Tensor, starts: torch.Tensor, drafts: torch.Tensor, uniform: torch.Tensor,
@@ -70,7 +70,7 @@ def verify(logits: torch.Tensor, starts: torch.Tensor, drafts: torch.Tensor, uni
     tokens = starts.new_empty((B, max_drafts + 1))      # int32; new_empty parses no options
     accepted, probs = starts.new_empty(B), noise.new_empty((B, max_drafts + 1))
     if B:
-        check(lib().esp_verify(logits.data_ptr(), code, stride, rows, vocab, at[0], B, at[1], at[2], n, q_ptr, q_code,
-                               q_stride, noise.data_ptr(), noise_stride, at[3] if len(at) > 3 else 0, max_drafts,
-                               tokens.data_ptr(), accepted.data_ptr(), probs.data_ptr(), stream_ptr(dev)))
+        launch(dev, lib().esp_verify, logits.data_ptr(), code, stride, rows, vocab, at[0], B, at[1], at[2], n, q_ptr, q_code,
+               q_stride, noise.data_ptr(), noise_stride, at[3] if len(at) > 3 else 0, max_drafts, tokens.data_ptr(),
+               accepted.data_ptr(), probs.data_ptr())
     return tokens, accepted, probs
