@@ -47,6 +47,7 @@ def test_launch_is_on_the_tensors_device(monkeypatch, make, current, device):
     entries = types.SimpleNamespace(esp_block_norm=note, esp_adapt=note, esp_verify=note)
     for module in (norms, adapters, speculative):
         monkeypatch.setattr(module, "lib", lambda: entries)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)      # (a GPU's would be looked for)
     monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: 4096)
     monkeypatch.setattr(torch.cuda, "device", on)
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: at[-1], raising=False)

@@ -358,8 +358,9 @@ def test_threads_of_different_widths(dev):
             assert refused == 0 and torch.equal(h, expected)
 
 
-def test_weights_on_another_device_are_refused():
+def test_weights_on_another_device_are_refused(monkeypatch):
     """No GPU needed: tensors without storage, refused before anything reads them."""
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)      # (a GPU's would be looked for)
     with FakeTensorMode():
         w = [torch.empty(64, device=f"cuda:{i}") for i in (0, 1)]
         for kw in (dict(pre=w[0], post=w[1]), dict(pre=w[0], pre_bias=w[1])):
