@@ -369,3 +369,19 @@ def test_weights_on_another_device_are_refused(monkeypatch):
         for kw in (dict(pre=w[1]), dict(post=w[1], pre=True), dict(pre=w[1], pre_bias=w[1])):
             with pytest.raises(ValueError, match="device|cuda:1"):
                 norms.BlockNorm(64, **kw)(torch.empty(2, 64, device="cuda:0"))
+
+
+@pytest.mark.gpu
+def test_rows_up_to_the_most_there_may_be(dev):
+    """2^31 - 1 rows of eight values, the same input in each: every one of them is written (34 GB), none past the last."""
+    rows, x = 2 ** 31 - 1, torch.arange(8, dtype=torch.bfloat16, device=dev)[None]
+    if torch.cuda.mem_get_info(dev)[0] < 40 << 30:
+        pytest.skip("less than 40 GB free")
+    buffer = torch.full((rows + 1, 8), -1.0, dtype=torch.bfloat16, device=dev)
+    norms.BlockNorm(8, block_scale=2.0)(x.expand(rows, 8), out=buffer[:rows])
+    words, want = buffer.view(torch.int64).view(-1, 2), (2 * x).view(torch.int64)
+    for at in range(0, rows, 1 << 28):
+        assert (words[at:min(at + (1 << 28), rows)] == want).all()
+    assert (buffer[rows] == -1).all()
+    with pytest.raises(EspError):
+        norms.BlockNorm(8)(x.expand(rows + 1, 8), out=x.expand(rows + 1, 8))

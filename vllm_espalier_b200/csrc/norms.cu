@@ -490,7 +490,7 @@ constexpr int RING_FIXED = 4 * 1024;            // of it, a CTA's barriers, scra
 constexpr int ring_ctas(int threads, int groups) { return groups > 1 ? 1 : threads >= 64 ? 1024 / threads : 16; }
 
 template <typename TX, typename TR, typename TW, int NT, int VPT>
-__global__ void __launch_bounds__(NT, ring_ctas(NT, VPT)) block_norm_ring(NormParams p, int rows, int stages) {
+__global__ void __launch_bounds__(NT, ring_ctas(NT, VPT)) block_norm_ring(NormParams p, unsigned rows, int stages) {
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ __align__(8) uint64_t full[MAX_STAGES];
     __shared__ __align__(16) float scratch[2][4][32];
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(NT, ring_ctas(NT, VPT)) block_norm_ring(NormPa
     __syncthreads();
     pdl_launch_dependents();
     pdl_wait();
-    const auto request = [&](int row, int s) {          // thread 0
+    const auto request = [&](unsigned row, int s) {         // thread 0
         uint32_t to = smem_addr(ring) + s * stage_bytes;
         mbar_arrive_expect_tx(&full[s], stage_bytes);
         bulk_g2s(to, static_cast<const TX*>(p.x) + row * p.x_stride, bx, &full[s]);
@@ -515,13 +515,14 @@ __global__ void __launch_bounds__(NT, ring_ctas(NT, VPT)) block_norm_ring(NormPa
         if (gate_rows) bulk_g2s(to, static_cast<const TX*>(p.gate) + row * p.gate_stride, bx, &full[s]), to += bx;
         if (p.residual) bulk_g2s(to, static_cast<const TR*>(p.residual) + row * p.residual_stride, br, &full[s]);
     };
-    const int step = gridDim.x;
+    // (unsigned: rows end below 2^31, and a row past the last by less than MAX_STAGES grids is still none)
+    const unsigned step = gridDim.x;
     if (tid == 0)
         for (int s = 0; s < stages && blockIdx.x + s * step < rows; ++s) request(blockIdx.x + s * step, s);
     RowWeights<TW, VEC, VPT> w;
     fetch_weights<TW, VEC, NT, VPT>(w, p);
     int s = 0, phase = 0, parity = 0;
-    for (int row = blockIdx.x; row < rows; row += step) {
+    for (unsigned row = blockIdx.x; row < rows; row += step) {
         // A wait that gave up ends the CTA, all threads together, after a bounded wait for the copies still on their way.
         if (!__syncthreads_and(mbar_wait(&full[s], phase))) {
             if (tid == 0)
@@ -530,8 +531,8 @@ __global__ void __launch_bounds__(NT, ring_ctas(NT, VPT)) block_norm_ring(NormPa
         }
         // that barrier also ends the row before: its stage can be filled again
         if (tid == 0 && row != blockIdx.x) {
-            const int last = (s ? s : stages) - 1, next = row + (stages - 1) * step;
-            if (next < rows) request(next, last);
+            const unsigned next = row + (stages - 1) * step;
+            if (next < rows) request(next, (s ? s : stages) - 1);
         }
         InStage<TX, TR, VEC> in;
         in.x_ = ring + s * stage_bytes;
@@ -554,7 +555,7 @@ bool vector_rows(const void* p, int dtype, long long stride) {
 
 struct RowsKernel {
     void (*run)(NormParams) = nullptr;
-    void (*ring)(NormParams, int, int) = nullptr;
+    void (*ring)(NormParams, unsigned, int) = nullptr;
     int threads = 0, ctas = 0;      // of a CTA; CTAs of the ring's kernel an SM
 };
 
@@ -665,7 +666,7 @@ extern "C" int esp_block_norm(const esp_block_norm_op_t* op, const void* x, long
             const int smem = stages * row_bytes(p);
             if (const int rc = allow_any_smem(k.ring, smem)) return rc;
             if (const int rc = launch(k.ring, dim3(k.ctas * device_sms()), dim3(k.threads), smem, stream, true, p,
-                                      static_cast<int>(rows), stages))
+                                      static_cast<unsigned>(rows), stages))
                 return rc;
             return ok();
         }
