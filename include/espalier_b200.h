@@ -374,8 +374,9 @@ int esp_block_norm(const esp_block_norm_op_t* op, const void* x, long long x_str
  * All arrays are device memory, contiguous and 16-byte aligned, a and b of the rows' dtype:
  *   a      [slots][n_mats][rank][k]       ranks  int32 [slots], or NULL: every slot has the full rank
  *   b      [slots][sum(widths)][rank]     scales fp32 [slots], or NULL: ones
- * rank is the capacity, a multiple of 8 up to 128; k and every width are multiples of 8; at most 4096 slots. A slot of rank q reads the
- * rows of a and the columns of b below q rounded up to 8 (those from q on hold zeros) and nothing past them.
+ * rank is the capacity, a multiple of 8 up to 128; k and every width are multiples of 8, k and their sum at most 2^30; at
+ * most 4096 slots. A slot of rank q reads the rows of a and the columns of b below q rounded up to 8 (those from q on hold
+ * zeros) and nothing past them.
  */
 typedef struct esp_adapters {
     const void *a, *b;
@@ -391,7 +392,7 @@ typedef struct esp_adapters {
  * id is outside [0, slots), or whose slot has rank 0, gets y[t]. x [t_rows][k], y and out [t_rows][sum(widths)] in
  * the adapters' dtype, rows 16-byte aligned (strides in elements, multiples of 8); out may be y itself. The inner
  * product is held in fp32 and the sum rounded once. A row's bits depend on its own id, x and y only.
- * ws: esp_adapt_ws_bytes(t_rows, slots) bytes of device memory, 16-byte aligned, of any content (NULL when that is 0).
+ * At most 2^26 rows. ws: esp_adapt_ws_bytes(t_rows, slots) bytes of device memory, 16-byte aligned, of any content (NULL when that is 0).
  */
 int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_stride, const void* y, long long y_stride,
               const int* ids, int t_rows, void* out, long long out_stride, void* ws, size_t ws_bytes, void* stream);
@@ -412,7 +413,7 @@ size_t esp_adapt_ws_bytes(int t_rows, int slots);
  * [requests] the number that stand; probs fp32 [requests][max_drafts + 1] p_i of each token (temperature 1 for a greedy
  * request), 0 after them. NaN logits count as -inf (a token ruled out); a row with nothing left gives -1 and ends the
  * request. A drafted id outside [0, vocab) never stands. Drafts past max_drafts are not looked at; a request whose
- * starts do not fit rows and n_drafts gets no token. Strides in elements; temperature NULL: 1, and one outside
+ * starts do not fit rows and n_drafts gets no token. vocab and max_drafts are at most 2^30. Strides in elements; temperature NULL: 1, and one outside
  * [1e-30, 1e30] counts as the nearer end.
  */
 int esp_verify(const void* logits, int dtype, long long stride, long long rows, int vocab, const int* starts,

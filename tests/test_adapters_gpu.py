@@ -12,6 +12,7 @@ from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from vllm_espalier_b200 import _lib, adapters
 
@@ -371,3 +372,26 @@ def test_threads_of_different_adapters(dev):
     with ThreadPoolExecutor(4) as pool:
         for (refused, out), expected in zip(pool.map(work, calls), want):
             assert refused == 0 and torch.equal(out, expected)
+
+
+def test_sizes_past_the_calls_integers_are_refused(monkeypatch):
+    """No GPU and no memory needed: shapes without storage."""
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    with FakeTensorMode():
+        e = lambda *s, t=torch.float16: torch.empty(*s, dtype=t, device="cuda:0")  # noqa: E731
+        ad = adapters.Adapters(e(1, 1, 8, 8), e(1, 8, 8), [8])
+        for rows in (2 ** 26 + 1, 2 ** 32 + 4):
+            with pytest.raises(ValueError, match="rows"):
+                ad(e(rows, 8), e(rows, 8), e(rows, t=torch.int32))
+        for k, n in ((2 ** 32 + 8, 8), (8, 2 ** 32 + 8), (2 ** 30 + 8, 8)):
+            with pytest.raises(ValueError, match="at most"):
+                adapters.Adapters(e(1, 1, 8, k), e(1, n, 8), [n])
+    ad = _lib.esp_adapters_t(16, 16, None, None, 1, 2, 8, 64, 1, (_lib.I * 4)(32))
+    for name, value in (("k", 2 ** 31 - 8), ("width", 2 ** 31 - 136)):
+        other = _lib.esp_adapters_t.from_buffer_copy(ad)
+        if name == "width":
+            other.widths[0] = value
+        else:
+            other.k = value
+        assert _lib.lib().esp_adapt(_lib.C.addressof(other), 16, 64, 16, 32, 16, 1, 16, 32, None, 0,
+                                    None) == _lib.ESP_ERR_INVALID, name

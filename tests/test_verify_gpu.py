@@ -12,6 +12,7 @@ import math
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from vllm_espalier_b200 import _lib
 from vllm_espalier_b200 import speculative
@@ -280,3 +281,17 @@ def test_library_refusals():
         assert lib.esp_verify(*dict(base, **change).values()) == _lib.ESP_ERR_INVALID, change
         assert lib.esp_last_error()
     assert lib.esp_verify(*dict(base, requests=0).values()) == _lib.ESP_OK
+
+
+def test_sizes_past_the_calls_integers_are_refused(monkeypatch):
+    """No GPU and no memory needed: shapes without storage."""
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    with FakeTensorMode():
+        i, f = (lambda n: torch.empty(n, dtype=torch.int32, device="cuda:0")), (lambda *n: torch.empty(*n, device="cuda:0"))
+        for B, V, drafts in ((1, 2 ** 32 + 5, 1), (1, 2 ** 30 + 1, 1), (1, 8, 2 ** 32 + 1), (1, 8, 2 ** 31 - 1),
+                             (2 ** 32 + 1, 8, 1)):
+            with pytest.raises(ValueError, match="up to"):
+                speculative.verify(f(B, V), i(B + 1), i(0), f(0), f(B, V), drafts)
+    for vocab, drafts in ((2 ** 31 - 1, 1), (2 ** 30 + 1, 1), (8, 2 ** 31 - 1)):
+        assert _lib.lib().esp_verify(16, 1, 8, 2, vocab, 16, 1, 16, 16, 1, None, 2, 8, 16, 8, None, drafts, 16, 16, 16,
+                                     None) == _lib.ESP_ERR_INVALID

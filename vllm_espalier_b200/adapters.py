@@ -18,6 +18,8 @@ from ._lib import DTYPE, esp_adapters_t, launch, lib
 
 MAX_RANK, MAX_MATS, MAX_SLOTS = 128, 4, 4096
 NONE = -1                     # the id of a row without an adapter
+MAX_ROWS = 1 << 26            # of one call
+MAX_COLUMNS = 1 << 30         # k, and the sum of the widths
 NO_PLAN = 64                  # rows up to which the kernel takes no workspace
 
 
@@ -42,6 +44,8 @@ class Adapters:
                              f"{MAX_MATS} matrices and {MAX_SLOTS} slots)")
         if rank % 8 or not 8 <= rank <= MAX_RANK or k % 8 or k < 8 or any(w % 8 or w < 8 for w in widths):
             raise ValueError(f"rank {rank} (8..{MAX_RANK}), k {k} and widths {widths} must be multiples of 8")
+        if k > MAX_COLUMNS or sum(widths) > MAX_COLUMNS:
+            raise ValueError(f"k {k} and {sum(widths)} columns must be {MAX_COLUMNS} at most")
         if not a.is_cuda or a.dtype not in (torch.float16, torch.bfloat16) or b.dtype != a.dtype:
             raise ValueError(f"a and b must be CUDA tensors, both fp16 or both bf16, got {a.dtype} and {b.dtype}")
         for name, t, dtype in (("b", b, a.dtype), ("ranks", ranks, torch.int32), ("scales", scales, torch.float32)):
@@ -123,6 +127,8 @@ class Adapters:
         rows = x.shape[0]
         if y.shape[0] != rows or ids.dim() != 1 or ids.numel() != rows:
             raise ValueError(f"x has {rows} rows, y {y.shape[0]}, ids {tuple(ids.shape)}")
+        if rows > MAX_ROWS:
+            raise ValueError(f"{rows} rows are more than {MAX_ROWS}")
         if ids.dtype != torch.int32 or ids.device != self.device or not ids.is_contiguous():
             raise ValueError(f"ids must be contiguous int32 on {self.device}, got {ids.dtype} on {ids.device}")
         if out is None:

@@ -830,14 +830,15 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
                 "esp_adapt: %d slots of %d matrices (1..%d slots, 1..4 matrices)", ad->slots, ad->n_mats, MAX_SLOTS);
     ESP_REQUIRE(ad->rank >= 8 && ad->rank <= 128 && ad->rank % 8 == 0, ESP_ERR_INVALID,
                 "esp_adapt: rank %d is not a multiple of 8 in 8..128", ad->rank);
-    ESP_REQUIRE(ad->k >= 8 && ad->k % 8 == 0, ESP_ERR_INVALID, "esp_adapt: k %d is not a multiple of 8", ad->k);
+    ESP_REQUIRE(ad->k >= 8 && ad->k % 8 == 0 && ad->k <= 1 << 30, ESP_ERR_INVALID,
+                "esp_adapt: k %d is not a multiple of 8 up to 2^30", ad->k);
     long long n = 0;
     for (int m = 0; m < ad->n_mats; ++m) {
         ESP_REQUIRE(ad->widths[m] >= 8 && ad->widths[m] % 8 == 0, ESP_ERR_INVALID,
                     "esp_adapt: width %d is not a multiple of 8", ad->widths[m]);
         n += ad->widths[m];
     }
-    ESP_REQUIRE(n < INT_MAX - 128, ESP_ERR_INVALID, "esp_adapt: %lld columns", n);
+    ESP_REQUIRE(n <= 1 << 30, ESP_ERR_INVALID, "esp_adapt: %lld columns (up to 2^30)", n);
     ESP_REQUIRE(t_rows >= 0 && t_rows <= (1 << 26), ESP_ERR_INVALID, "esp_adapt: %d rows", t_rows);
     if (t_rows == 0) return ok();
     ESP_REQUIRE(ad->a && ad->b && x && y && ids && out, ESP_ERR_INVALID, "esp_adapt: null pointer");

@@ -607,6 +607,8 @@ auto kernel_of(bool given, int probs_dtype) {
     return probs_dtype == BF16 ? verify_kernel<T, __nv_bfloat16> : verify_kernel<T, __half>;
 }
 
+constexpr int MAX_COUNT = 1 << 30;
+
 bool known_dtype(int t) { return t == F16 || t == BF16 || t == F32; }
 
 }  // namespace
@@ -623,7 +625,9 @@ extern "C" int esp_verify(const void* logits, int dtype, long long stride, long 
     ESP_REQUIRE(known_dtype(dtype), ESP_ERR_INVALID, "esp_verify: unknown logits dtype %d", dtype);
     ESP_REQUIRE(requests >= 0 && rows >= 0 && n_drafts >= 0 && max_drafts >= 0, ESP_ERR_INVALID,
                 "esp_verify: negative size");
-    ESP_REQUIRE(vocab >= 1, ESP_ERR_INVALID, "esp_verify: vocabulary of %d", vocab);
+    // (ids and places are int, up to a batch of loads past the last)
+    ESP_REQUIRE(vocab >= 1 && vocab <= MAX_COUNT && max_drafts <= MAX_COUNT, ESP_ERR_INVALID,
+                "esp_verify: vocabulary of %d, %d drafted tokens (1..2^30, up to 2^30)", vocab, max_drafts);
     if (requests == 0) return ok();
     ESP_REQUIRE(logits && starts && noise && tokens && accepted && probs, ESP_ERR_INVALID, "esp_verify: null pointer");
     ESP_REQUIRE(n_drafts == 0 || (drafts && uniform), ESP_ERR_INVALID, "esp_verify: drafted tokens without a pointer");

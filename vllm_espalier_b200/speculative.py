@@ -14,6 +14,8 @@ import torch
 
 from ._lib import DTYPE, launch, lib
 
+MAX_COUNT = 1 << 30           # requests, ids of the vocabulary, drafted tokens of a request
+
 
 def verify(logits: torch.Tensor, starts: torch.Tensor, drafts: torch.Tensor, uniform: torch.Tensor,
            noise: torch.Tensor, max_drafts: int, temperature: torch.Tensor | None = None,
@@ -38,8 +40,9 @@ def verify(logits: torch.Tensor, starts: torch.Tensor, drafts: torch.Tensor, uni
     if n < 0 or (B == 0 and n > 0):
         raise ValueError(f"{rows} rows of logits for {B} requests: every request has a row for each drafted token "
                          "and one more")
-    if vocab < 1 or max_drafts < 0:
-        raise ValueError(f"a vocabulary of {vocab} and at most {max_drafts} drafted tokens")
+    if not (B <= MAX_COUNT and 1 <= vocab <= MAX_COUNT and 0 <= max_drafts <= MAX_COUNT):
+        raise ValueError(f"{B} requests, a vocabulary of {vocab} and at most {max_drafts} drafted tokens (each up to "
+                         f"{MAX_COUNT})")
     flat = [("starts", starts, B + 1, torch.int32), ("drafts", drafts, n, torch.int32),
             ("uniform", uniform, n, torch.float32)]
     if temperature is not None:
