@@ -395,3 +395,21 @@ def test_sizes_past_the_calls_integers_are_refused(monkeypatch):
             other.k = value
         assert _lib.lib().esp_adapt(_lib.C.addressof(other), 16, 64, 16, 32, 16, 1, 16, 32, None, 0,
                                     None) == _lib.ESP_ERR_INVALID, name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rank", [16, 32, 64, 128])
+@pytest.mark.parametrize("T", [1, 50, 1100])
+def test_inner_products_are_held_in_fp32(dev, dtype, rank, T):
+    """Two inner products whose leading 20 bits cancel in the output: every product and sum is exact in fp32, so 2^-20
+    comes out, and nothing where the inner products are held in fewer than 21 bits."""
+    ad = adapters.Adapters(torch.zeros(1, 1, rank, 256, dtype=dtype, device=dev),
+                           torch.zeros(1, 64, rank, dtype=dtype, device=dev), [64])
+    x = torch.zeros(T, 256, dtype=dtype, device=dev)
+    x[:, [3, 100, 200]] = 1
+    for r, values in ((1, (1, 2.0 ** -9, 2.0 ** -20)), (6, (-1, -2.0 ** -9, 0))):
+        ad.a[0, 0, r, [3, 100, 200]] = torch.tensor(values, device=dev).to(dtype)
+        ad.b[0, :, r] = 1
+    got = ad(x, torch.zeros(T, 64, dtype=dtype, device=dev), torch.zeros(T, dtype=torch.int32, device=dev))
+    assert (got == 2.0 ** -20).all(), got.unique()

@@ -13,9 +13,9 @@
 // The products are small (rank 16: 35 flops a byte), so bytes bound a large batch and latency a small one. mma.sync and not
 // tcgen05: the tensor pipe is 6 to 17% busy, u is born in registers and goes back into them, and both paths share one order
 // of summation. Measured (q | k | v of 2048 -> 5120, rank 16 unless said): one token 5.8 us (ids, one round trip to A, two
-// cluster barriers, one to B and y), 48 rows of 64 adapters of rank 32 13.8 us, 8192 rows of 12 prompts 57 us = 3.6 TB/s
-// (55% of a plain copy; plan 4 us, the rest is stage hand-overs), 3001 rows at rank 64 73 us (17%: two halves of u double
-// the products, and sums, halves and ring leave one CTA an SM).
+// cluster barriers, one to B and y), 48 rows of 64 adapters of rank 32 14 us, 8192 rows of 12 prompts 61 us = 3.3 TB/s
+// (52% of a plain copy; plan 4 us, the rest is stage hand-overs), 3001 rows at rank 64 82 us (15%: the parts that hold u in
+// fp32 treble the second product, and sums or parts and the ring leave one CTA an SM).
 #include <cuda_runtime.h>
 
 #include <limits.h>
@@ -164,26 +164,32 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
 // What both kernels below share. Inner columns of a tile: RP = 16 RANK16 a matrix (the capacity in steps of 16), u of all
 // matrices side by side.
 // ---------------------------------------------------------------------------------------------------------------
-// Elements between rows of u's halves: 64 bytes past a multiple of 128, so that the eight lanes of a quarter load meet
+// u's parts of 16 bits each, which add up to it: three of bf16's 8 bits hold an fp32 sum's 24, two of fp16's 11 with their
+// rounding to nearest miss at most its last one.
+template <typename T>
+constexpr int PARTS = std::is_same_v<T, __half> ? 2 : 3;
+
+// Elements between rows of u's parts: 64 bytes past a multiple of 128, so that the eight lanes of a quarter load meet
 // every bank once.
 __host__ __device__ constexpr int u_stride(int cols) { return cols + (192 - cols * 2 % 128) % 128 / 2; }
 
-// Shared memory of a tile: sums [M][cols] fp32 of this CTA, then u_hi and u_lo [M][stride] 16-bit and the rows' factors.
+// Shared memory of a tile: sums [M][cols] fp32 of this CTA, then (or over them) u's parts [PARTS][M][stride] and the rows'
+// factors.
 template <typename T>
 struct Inner {
     float* sums;
-    T *hi, *lo;
+    T* part;
     float* factor;
-    int cols, stride;
-    __device__ __forceinline__ Inner(unsigned char* at, int m, int cols_) : cols(cols_), stride(u_stride(cols_)) {
+    int cols, stride, part_size;        // elements from a row and from a part to the next
+    __device__ __forceinline__ Inner(unsigned char* at, int m, int cols_, bool over)
+        : cols(cols_), stride(u_stride(cols_)), part_size(m * stride) {
         sums = reinterpret_cast<float*>(at);
-        hi = reinterpret_cast<T*>(sums + m * cols);
-        lo = hi + m * stride;
-        factor = reinterpret_cast<float*>(lo + m * stride);
+        part = reinterpret_cast<T*>(over ? sums : sums + m * cols);
+        factor = reinterpret_cast<float*>(part + PARTS<T> * part_size);
     }
 };
 constexpr int sums_bytes(int m, int cols) { return m * cols * 4; }
-constexpr int halves_bytes(int m, int cols) { return m * (2 * u_stride(cols) * 2 + 4); }
+constexpr int parts_bytes(int m, int cols, int parts) { return m * (parts * u_stride(cols) * 2 + 4); }
 
 // The adapter of a slot: its rank in whole steps of 8 (0: nothing to add), its matrices.
 template <typename T>
@@ -244,19 +250,13 @@ __device__ __forceinline__ void copy_rows(const AdaptParams& p, const int* tile_
                 reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + tile_rows[r] * p.y_stride)[c];
 }
 
-// Join the cluster's sums of one row (a warp) as the tree over the segments and store it into every CTA as two 16-bit
-// halves (hi + lo is the sum to 2^-16 of it, so the second product rounds nothing that the output shows). For fp16 a row
-// is first scaled by a power of two that brings its largest value to [2^14, 2^15); the factor comes back with the
-// adapter's scale.
+// The cluster's sums of one row (a warp), joined as the tree over the segments: a lane's columns 2 lane + 64 i and the next.
 template <typename T, int RANK16, int CTAS>
-__device__ __forceinline__ void join_row(const Inner<T>& u, int r, int r8, float scale) {
+__device__ __forceinline__ void join_row(const Inner<T>& u, int r, int r8, float2 (&v)[RANK16]) {
     constexpr int RP = RANK16 * 16;
-    const int lane = threadIdx.x % 32;
-    float2 v[RANK16];
-    float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < RANK16; ++i) {
-        const int c = lane * 2 + i * 64;
+        const int c = threadIdx.x % 32 * 2 + i * 64;
         v[i] = {0.0f, 0.0f};
         if (c < u.cols && c % RP < r8) {
             float2 o[CTAS];
@@ -268,10 +268,20 @@ __device__ __forceinline__ void join_row(const Inner<T>& u, int r, int r8, float
                 for (int w = 0; w < CTAS; w += 2 * n) o[w].x += o[w + n].x, o[w].y += o[w + n].y;
             v[i] = o[0];
         }
-        top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
     }
+}
+
+// Store it into every CTA as its parts, so that the second product holds it in fp32 as the sum had it. For fp16 a row is
+// first scaled by a power of two that brings its largest value to [2^14, 2^15); the factor comes back with the adapter's
+// scale.
+template <typename T, int RANK16, int CTAS>
+__device__ __forceinline__ void store_row(const Inner<T>& u, int r, const float2 (&v)[RANK16], float scale) {
+    const int lane = threadIdx.x % 32;
     float up = 1.0f, down = scale;
     if constexpr (std::is_same_v<T, __half>) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < RANK16; ++i) top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
         top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
         if (top > 1e-30f && top < 1e30f) {
             const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
@@ -283,15 +293,15 @@ __device__ __forceinline__ void join_row(const Inner<T>& u, int r, int r8, float
     for (int i = 0; i < RANK16; ++i) {
         const int c = lane * 2 + i * 64;
         if (c >= u.cols) continue;
-        const float a = v[i].x * up, b = v[i].y * up;
-        const uint32_t hi = pack(a, b, T());
-        const float2 back = unpack(hi, T());
-        // (an infinite half leaves nothing to the other one)
-        const uint32_t lo = pack(isinf(back.x) ? 0.0f : a - back.x, isinf(back.y) ? 0.0f : b - back.y, T());
+        float a = v[i].x * up, b = v[i].y * up;
 #pragma unroll
-        for (int w = 0; w < CTAS; ++w) {
-            st_cluster_u32(u.hi + r * u.stride + c, w, hi);
-            st_cluster_u32(u.lo + r * u.stride + c, w, lo);
+        for (int k = 0; k < PARTS<T>; ++k) {
+            const uint32_t bits = pack(a, b, T());
+            const float2 back = unpack(bits, T());
+            // (an infinite part leaves nothing to the others)
+            a = isinf(back.x) ? 0.0f : a - back.x, b = isinf(back.y) ? 0.0f : b - back.y;
+#pragma unroll
+            for (int w = 0; w < CTAS; ++w) st_cluster_u32(u.part + k * u.part_size + r * u.stride + c, w, bits);
         }
     }
     if (lane < CTAS) st_cluster_u32(u.factor + r, lane, __float_as_uint(down));
@@ -313,27 +323,25 @@ __device__ __forceinline__ void u_fragments(const T* u, int stride, int s, int q
 
 // u times a block of B into acc. The four n8 tiles of a block take columns so that a lane ends up with eight consecutive
 // ones: tile j's column c is 8 (c / 2) + 2 j + c % 2 of the block; w(j, s) gives the lane's values of B's row for its
-// column g of tile j (eight of steps s and s + 1; four of the one step of RANK16 1).
+// column g of tile j (eight of steps s and s + 1; four of the one step of RANK16 1). The order of the products that meet in
+// a value: two steps of the first part, of the second, ..., the next two steps.
 template <typename T, int RANK16, typename W>
-__device__ __forceinline__ void second_product(float (&acc)[4][4], const T* hi_at, const T* lo_at, int stride, int r8, int q,
-                                               W w) {
-    uint32_t hi[2][4], lo[2][4];
+__device__ __forceinline__ void second_product(float (&acc)[4][4], const Inner<T>& u, int at, int r8, int q, W w) {
 #pragma unroll
     for (int s = 0; s < RANK16; s += 2) {
         if (s * 16 >= r8) break;
         uint4 k[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) k[j] = w(j, s);
-        u_fragments<RANK16>(hi_at, stride, s, q, hi);
-        u_fragments<RANK16>(lo_at, stride, s, q, lo);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            mma<T>(acc[j], hi[0], k[j].x, k[j].y);
-            mma<T>(acc[j], lo[0], k[j].x, k[j].y);
-            if constexpr (RANK16 > 1) {
-                mma<T>(acc[j], hi[1], k[j].z, k[j].w);
-                mma<T>(acc[j], lo[1], k[j].z, k[j].w);
-            }
+        for (int i = 0; i < PARTS<T>; ++i) {
+            uint32_t f[2][4];
+            u_fragments<RANK16>(u.part + i * u.part_size + at, u.stride, s, q, f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma<T>(acc[j], f[0], k[j].x, k[j].y);
+            if constexpr (RANK16 > 1)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma<T>(acc[j], f[1], k[j].z, k[j].w);
         }
     }
 }
@@ -366,7 +374,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) adapt_few(AdaptParams p) {
     __shared__ int tile_slot, tile_count, found;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
     const int rank = blockIdx.x % FEW_CTAS, tile = blockIdx.x / FEW_CTAS;
-    const Inner<T> u(smem, M, p.ad.n_mats * RP);
+    const Inner<T> u(smem, M, p.ad.n_mats * RP, false);
     pdl_launch_dependents();
     pdl_wait();
 
@@ -466,8 +474,11 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) adapt_few(AdaptParams p) {
     else first_product(std::integral_constant<int, 3>(), std::integral_constant<int, 4>());
     cluster_sync_all();
     const float scale = p.ad.scales ? p.ad.scales[slot] : 1.0f;
-    for (int r = rank * (M / FEW_CTAS) + warp; r < (rank + 1) * (M / FEW_CTAS); r += WARPS)
-        join_row<T, RANK16, FEW_CTAS>(u, r, ad.r8, scale);
+    for (int r = rank * (M / FEW_CTAS) + warp; r < (rank + 1) * (M / FEW_CTAS); r += WARPS) {
+        float2 v[RANK16];
+        join_row<T, RANK16, FEW_CTAS>(u, r, ad.r8, v);
+        store_row<T, RANK16, FEW_CTAS>(u, r, v, scale);
+    }
     cluster_sync_all();     // (the last access to another CTA's memory was before it)
 
     const float fa = u.factor[g], fb = u.factor[g + 8];
@@ -479,8 +490,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) adapt_few(AdaptParams p) {
         const uint4 yb = in && rb >= 0 ? *reinterpret_cast<const uint4*>(y + rb * p.y_stride + col) : zero;
         const T* w = ad.b + (static_cast<size_t>(block.col) + (g >> 1) * 8 + (g & 1)) * ad.cap;
         float acc[4][4] = {};
-        const size_t at = g * u.stride + block.m * RP;
-        second_product<T, RANK16>(acc, u.hi + at, u.lo + at, u.stride, ad.r8, q, [&](int j, int s) {
+        second_product<T, RANK16>(acc, u, g * u.stride + block.m * RP, ad.r8, q, [&](int j, int s) {
             if constexpr (RANK16 == 1) {
                 const uint2 v = n_in && q * 4 < ad.r8 ? *reinterpret_cast<const uint2*>(w + j * 2 * ad.cap + q * 4) : uint2{0, 0};
                 return uint4{v.x, v.y, 0, 0};
@@ -510,9 +520,15 @@ constexpr int stage_bytes(int cols, int rank16) {
     const int first = (MANY_ROWS + cols) * 128, second = MANY_ROWS * 256 + 128 * rank16 * 32;
     return first > second ? first : second;
 }
-constexpr int many_bytes(int cols, int rank16, int stages, int ctas) {
-    const int levels = (ctas >= 4 ? 1 : 2) * sums_bytes(MANY_ROWS, cols), halves = halves_bytes(MANY_ROWS, cols);
-    return stages * stage_bytes(cols, rank16) + sums_bytes(MANY_ROWS, cols) + (ctas < 8 && levels > halves ? levels : halves);
+// From rank 33 on u's three parts of bf16 go over the sums and their levels, once every CTA has read them: beside them the
+// ring would not have its three stages. That costs a cluster barrier, which fp16's two parts do not need (3001 x rank 64:
+// 73 us without it, 74 with it).
+constexpr bool parts_over(int rank16, int parts) { return rank16 >= 4 && parts > 2; }
+constexpr int many_bytes(int cols, int rank16, int stages, int ctas, int parts) {
+    const int sums = sums_bytes(MANY_ROWS, cols), levels = ctas >= 8 ? 0 : (ctas >= 4 ? 1 : 2) * sums;
+    const int u = parts_bytes(MANY_ROWS, cols, parts);
+    const int inner = parts_over(rank16, parts) ? (sums + levels > u ? sums + levels : u) : sums + (levels > u ? levels : u);
+    return stages * stage_bytes(cols, rank16) + inner;
 }
 
 template <typename T, int RANK16, int CTAS>
@@ -525,7 +541,7 @@ __global__ void __launch_bounds__(many_warps(RANK16) * 32, RANK16 >= 4 ? 1 : 2) 
     const int row_warp = warp % GROUPS, col_warp = warp / GROUPS;
     const int rank = blockIdx.x % CTAS, tile = blockIdx.x / CTAS;
     const int cols = p.ad.n_mats * RP, slot_bytes = stage_bytes(cols, RANK16);
-    const Inner<T> u(smem + stages * slot_bytes, M, cols);
+    const Inner<T> u(smem + stages * slot_bytes, M, cols, parts_over(RANK16, PARTS<T>));
     pdl_launch_dependents();
     pdl_wait();
     const Tile mine = reinterpret_cast<const Tile*>(p.plan)[tile];
@@ -642,10 +658,10 @@ __global__ void __launch_bounds__(many_warps(RANK16) * 32, RANK16 >= 4 ? 1 : 2) 
     };
 
     // u = x A^T, a segment at a time; sums of segments join as the tree's levels complete (level l of this thread's values
-    // in shared memory, where u's halves will be).
+    // in shared memory).
     const int per = (ad.n_tiles + 3) / 4, t0 = col_warp * per, nt = min(per, ad.n_tiles - t0);
     const int la = row_warp * 16 * F + g;       // the first of this lane's rows: la + 16 f and la + 16 f + 8
-    float* levels = reinterpret_cast<float*>(u.hi);
+    float* levels = u.sums + M * cols;      // (where u's parts will be)
     // lane (g, q)'s piece of half h of an even or odd row: q or q + 4
     const uint32_t x_at = la * 128 + q * 16, a_at = (M + t0 * 8 + g) * 128 + q * 16, odd = (g & 1) * 64;
 #pragma unroll
@@ -701,8 +717,24 @@ __global__ void __launch_bounds__(many_warps(RANK16) * 32, RANK16 >= 4 ? 1 : 2) 
     }
     cluster_sync_all();
     const float scale = p.ad.scales ? p.ad.scales[mine.slot] : 1.0f;
-    for (int r = rank * (M / CTAS) + warp; r < (rank + 1) * (M / CTAS); r += WARPS)
-        join_row<T, RANK16, CTAS>(u, r, ad.r8, scale);
+    if constexpr (parts_over(RANK16, PARTS<T>)) {
+        constexpr int ROWS = (M / CTAS + WARPS - 1) / WARPS;
+        float2 v[ROWS][RANK16];
+        const auto row = [&](int i) { return warp + i * WARPS < M / CTAS ? rank * (M / CTAS) + warp + i * WARPS : -1; };
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+            if (row(i) >= 0) join_row<T, RANK16, CTAS>(u, row(i), ad.r8, v[i]);
+        cluster_sync_all();
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+            if (row(i) >= 0) store_row<T, RANK16, CTAS>(u, row(i), v[i], scale);
+    } else {
+        for (int r = rank * (M / CTAS) + warp; r < (rank + 1) * (M / CTAS); r += WARPS) {
+            float2 v[RANK16];
+            join_row<T, RANK16, CTAS>(u, r, ad.r8, v);
+            store_row<T, RANK16, CTAS>(u, r, v, scale);
+        }
+    }
     cluster_sync_all();     // (the last access to another CTA's memory was before it)
 
     T* to[F][2];
@@ -717,23 +749,18 @@ __global__ void __launch_bounds__(many_warps(RANK16) * 32, RANK16 >= 4 ? 1 : 2) 
         }
     const uint32_t y_at = la * 256 + (col_warp * 4 + q ^ (g & 1) << 2) * 16;
     const uint32_t b_at = M * 256 + (col_warp * 32 + g) * ROW * 16;
-    const uint32_t row_bytes = u.stride * sizeof(T), u_at = smem_addr(u.hi) + la * row_bytes, lo_off = M * row_bytes;
-    // hi and lo of steps s and s + 1 of row fragment f, for the matrix whose halves start at `at`
-    const auto fragments = [&](uint32_t at, int f, int s, uint32_t (&hi)[2][4], uint32_t (&lo)[2][4]) {
+    const uint32_t row_bytes = u.stride * sizeof(T), u_at = smem_addr(u.part) + la * row_bytes, part_bytes = M * row_bytes;
+    // steps s and s + 1 of row fragment f, for the matrix and part that start at `at`
+    const auto fragment = [&](uint32_t at, int f, int s, uint32_t (&o)[2][4]) {
         const uint32_t a = at + f * 16 * row_bytes, b = a + 8 * row_bytes;
         if constexpr (RANK16 == 1) {
             const uint2 h0 = ld_shared_v2(a + q * 8), h1 = ld_shared_v2(b + q * 8);
-            const uint2 l0 = ld_shared_v2(a + lo_off + q * 8), l1 = ld_shared_v2(b + lo_off + q * 8);
-            hi[0][0] = h0.x, hi[0][1] = h1.x, hi[0][2] = h0.y, hi[0][3] = h1.y;
-            lo[0][0] = l0.x, lo[0][1] = l1.x, lo[0][2] = l0.y, lo[0][3] = l1.y;
+            o[0][0] = h0.x, o[0][1] = h1.x, o[0][2] = h0.y, o[0][3] = h1.y;
         } else {
             const uint32_t off = s * 32 + q * 16;
             const uint4 h0 = ld_shared_v4(a + off), h1 = ld_shared_v4(b + off);
-            const uint4 l0 = ld_shared_v4(a + lo_off + off), l1 = ld_shared_v4(b + lo_off + off);
-            hi[0][0] = h0.x, hi[0][1] = h1.x, hi[0][2] = h0.y, hi[0][3] = h1.y;
-            hi[1][0] = h0.z, hi[1][1] = h1.z, hi[1][2] = h0.w, hi[1][3] = h1.w;
-            lo[0][0] = l0.x, lo[0][1] = l1.x, lo[0][2] = l0.y, lo[0][3] = l1.y;
-            lo[1][0] = l0.z, lo[1][1] = l1.z, lo[1][2] = l0.w, lo[1][3] = l1.w;
+            o[0][0] = h0.x, o[0][1] = h1.x, o[0][2] = h0.y, o[0][3] = h1.y;
+            o[1][0] = h0.z, o[1][1] = h1.z, o[1][2] = h0.w, o[1][3] = h1.w;
         }
     };
     for (int i = 0; i < n_second; ++i) {
@@ -760,20 +787,17 @@ __global__ void __launch_bounds__(many_warps(RANK16) * 32, RANK16 >= 4 ? 1 : 2) 
                 }
             }
 #pragma unroll
-            for (int f = 0; f < F; ++f) {
-                uint32_t hi[2][4], lo[2][4];
-                fragments(u_m, f, s, hi, lo);
+            for (int f = 0; f < F; ++f)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mma<T>(acc[f][j], hi[0], w[j].x, w[j].y);
+                for (int k = 0; k < PARTS<T>; ++k) {        // (in second_product's order)
+                    uint32_t v[2][4];
+                    fragment(u_m + k * part_bytes, f, s, v);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mma<T>(acc[f][j], lo[0], w[j].x, w[j].y);
-                if constexpr (RANK16 > 1) {
+                    for (int j = 0; j < 4; ++j) mma<T>(acc[f][j], v[0], w[j].x, w[j].y);
+                    if constexpr (RANK16 > 1)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mma<T>(acc[f][j], hi[1], w[j].z, w[j].w);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mma<T>(acc[f][j], lo[1], w[j].z, w[j].w);
+                        for (int j = 0; j < 4; ++j) mma<T>(acc[f][j], v[1], w[j].z, w[j].w);
                 }
-            }
         }
         if (q * 8 >= block.left) continue;
 #pragma unroll
@@ -809,6 +833,7 @@ int rank_steps(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ?
 long long max_tiles(int rows, int slots, int m) { return (rows + m - 1) / m + (rows < slots + 1 ? rows : slots + 1); }
 
 constexpr int MAX_SMEM = 226 * 1024;    // a CTA's dynamic shared memory, beside its few static words
+constexpr int HALF_SM = 112 * 1024 + 512;       // the same where two CTAs share an SM's 228 KB (1 KB of a CTA is the system's)
 constexpr double CTA_COST = 0.06;       // of a tile's work, what a CTA spends on joining sums whatever its share is
 
 }  // namespace
@@ -851,6 +876,7 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
 
     const int steps = rank_steps(ad->rank), cols = ad->n_mats * steps * 16;
     const bool half = ad->dtype == F16;
+    const int parts = half ? PARTS<__half> : PARTS<__nv_bfloat16>;
     // Tiles of 64 rows where the inner columns fit a CTA, tiles of 16 need more than two rounds of the GPU's clusters, and
     // adapters have enough rows each that tiles of 64 are not mostly empty. Measured, 16 / 64 rows a tile, us, rank 16, 32 and
     // 64: 512 rows 15 / 17, 18 / 23, 22 / 24; 1024 rows 21 / 20, 26 / 27, 34 / 39; 1536 rows 30 / 21, 37 / 28, 49 / 39. 64
@@ -869,7 +895,7 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
     }
     if (!many) {
         const auto kernel = half ? few_kernel<__half>(steps) : few_kernel<__nv_bfloat16>(steps);
-        const size_t smem = sums_bytes(m, cols) + halves_bytes(m, cols);
+        const size_t smem = sums_bytes(m, cols) + parts_bytes(m, cols, parts);
         if (const int rc = allow_any_smem(kernel, smem)) return rc;
         if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * FEW_CTAS), dim3(FEW_WARPS * 32),
                                           smem, stream, true, FEW_CTAS, p))
@@ -879,23 +905,23 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
     // CTAs a tile: what takes the least rounds x (a CTA's share of a tile + what it spends on joining sums). Places: two CTAs
     // an SM (one from rank 33 on, or where a ring of two stages does not fit twice), as many whole clusters as the 18 SMs of a
     // GPC hold. Measured: 128 tiles of rank 16 with 2 / 4 / 8 CTAs 68 / 74 / 90 us, 47 tiles of rank 64 with 4 / 8 75 / 85 us.
-    const int half_sm = MAX_SMEM / 2 - 1024, tiles = (t_rows + m - 1) / m + std::min(ad->slots, t_rows / m) / 2;
+    const int half_sm = HALF_SM, tiles = (t_rows + m - 1) / m + std::min(ad->slots, t_rows / m) / 2;
     int ctas = 8;       // (fits whatever fits at all)
     double best = 1e30;
     for (int c : {2, 4, 8}) {
-        if (many_bytes(cols, steps, 3, c) > MAX_SMEM) continue;
-        const int an_sm = steps < 4 && many_bytes(cols, steps, steps == 2 ? 2 : 3, c) <= half_sm ? 2 : 1;
+        if (many_bytes(cols, steps, 3, c, parts) > MAX_SMEM) continue;
+        const int an_sm = steps < 4 && many_bytes(cols, steps, steps == 2 ? 2 : 3, c, parts) <= half_sm ? 2 : 1;
         const int places = std::max(device_sms() / 18, 1) * (18 * an_sm / c) * c;
         const double work = ((tiles * c + places - 1) / places) * (1.0 / c + CTA_COST);
         if (work < best) best = work, ctas = c;
     }
     // Two stages where that leaves an SM to two CTAs: q | k | v at rank 32, 8192 rows 97 us against 125 with three and one CTA.
-    const bool three = steps != 2 || many_bytes(cols, steps, 3, ctas) <= half_sm;
-    const int least = three || many_bytes(cols, steps, 2, ctas) > half_sm ? 3 : 2;
-    const int room = steps < 4 && many_bytes(cols, steps, least, ctas) <= half_sm ? half_sm : MAX_SMEM;
+    const bool three = steps != 2 || many_bytes(cols, steps, 3, ctas, parts) <= half_sm;
+    const int least = three || many_bytes(cols, steps, 2, ctas, parts) > half_sm ? 3 : 2;
+    const int room = steps < 4 && many_bytes(cols, steps, least, ctas, parts) <= half_sm ? half_sm : MAX_SMEM;
     int stages = 4;
-    while (stages > least && many_bytes(cols, steps, stages, ctas) > room) --stages;
-    const size_t smem = many_bytes(cols, steps, stages, ctas);
+    while (stages > least && many_bytes(cols, steps, stages, ctas, parts) > room) --stages;
+    const size_t smem = many_bytes(cols, steps, stages, ctas, parts);
     const auto kernel = half ? many_kernel<__half>(steps, ctas) : many_kernel<__nv_bfloat16>(steps, ctas);
     if (const int rc = allow_any_smem(kernel, smem)) return rc;
     if (const int rc = launch_cluster(kernel, dim3(static_cast<unsigned>(p.max_tiles) * ctas), dim3(many_warps(steps) * 32), smem,
