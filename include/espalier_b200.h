@@ -390,9 +390,10 @@ typedef struct esp_adapters {
 /*
  * out[t] = y[t] + scales[a] * (x[t] A[a, s]^T) B[a, s]^T for every matrix s, a = ids[t] (int32 [t_rows]); a row whose
  * id is outside [0, slots), or whose slot has rank 0, gets y[t]. x [t_rows][k], y and out [t_rows][sum(widths)] in
- * the adapters' dtype, rows 16-byte aligned (strides in elements, multiples of 8); out may be y itself. The inner
- * product is held in fp32 and the sum rounded once. A row's bits depend on its own id, x and y only.
- * At most 2^26 rows. ws: esp_adapt_ws_bytes(t_rows, slots) bytes of device memory, 16-byte aligned, of any content (NULL when that is 0).
+ * the adapters' dtype, rows 16-byte aligned (strides in elements, multiples of 8); out may be y itself. At most 2^26 rows.
+ * The inner product x A^T is held in fp32 (fp16: to 24 bits from 2^-15 of the row's and matrix's largest up, smaller ones to
+ * 2^-39 of that) and the sum is rounded once. A row's bits depend on its own id, x and y only.
+ * ws: esp_adapt_ws_bytes(t_rows, slots) bytes of device memory, 16-byte aligned, of any content (NULL when that is 0).
  */
 int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_stride, const void* y, long long y_stride,
               const int* ids, int t_rows, void* out, long long out_stride, void* ws, size_t ws_bytes, void* stream);

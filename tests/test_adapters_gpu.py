@@ -413,3 +413,18 @@ def test_inner_products_are_held_in_fp32(dev, dtype, rank, T):
         ad.b[0, :, r] = 1
     got = ad(x, torch.zeros(T, 64, dtype=dtype, device=dev), torch.zeros(T, dtype=torch.int32, device=dev))
     assert (got == 2.0 ** -20).all(), got.unique()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("widths", [[64, 40], [32, 40, 64], [32, 32, 32, 64]])
+@pytest.mark.parametrize("rank", [8, 16, 32, 64, 128])
+@pytest.mark.parametrize("T", [3, 1100])
+def test_a_large_matrix_leaves_the_others_their_digits_in_fp16(dev, widths, rank, T):
+    """Inner products of the first matrix 2^30 times those of the others: each keeps 2^-16 of itself."""
+    ad = make(dev, torch.float16, 256, widths, 2, rank, 5, ranks=[rank, rank])
+    ad.a[:, 0].mul_(2.0 ** 14)
+    ad.a[:, 1:].mul_(2.0 ** -16)
+    ad.b[:, :widths[0]].mul_(2.0 ** -8)
+    ad.b[:, widths[0]:].mul_(2.0 ** 11)
+    x, y, i = rows(dev, ad, T, 4)
+    check(ad(x, y.zero_(), i), ad, x, y, i)

@@ -173,8 +173,8 @@ constexpr int PARTS = std::is_same_v<T, __half> ? 2 : 3;
 // every bank once.
 __host__ __device__ constexpr int u_stride(int cols) { return cols + (192 - cols * 2 % 128) % 128 / 2; }
 
-// Shared memory of a tile: sums [M][cols] fp32 of this CTA, then (or over them) u's parts [PARTS][M][stride] and the rows'
-// factors.
+// Shared memory of a tile: sums [M][cols] fp32 of this CTA, then (or over them) u's parts [PARTS][M][stride] and, of fp16, the
+// factors [M][4] of a row's matrices.
 template <typename T>
 struct Inner {
     float* sums;
@@ -189,7 +189,7 @@ struct Inner {
     }
 };
 constexpr int sums_bytes(int m, int cols) { return m * cols * 4; }
-constexpr int parts_bytes(int m, int cols, int parts) { return m * (parts * u_stride(cols) * 2 + 4); }
+constexpr int parts_bytes(int m, int cols, int parts) { return m * (parts * u_stride(cols) * 2 + (parts == 2 ? 16 : 0)); }
 
 // The adapter of a slot: its rank in whole steps of 8 (0: nothing to add), its matrices.
 template <typename T>
@@ -271,29 +271,44 @@ __device__ __forceinline__ void join_row(const Inner<T>& u, int r, int r8, float
     }
 }
 
-// Store it into every CTA as its parts, so that the second product holds it in fp32 as the sum had it. For fp16 a row is
-// first scaled by a power of two that brings its largest value to [2^14, 2^15); the factor comes back with the adapter's
-// scale.
+// Store it into every CTA as its parts, so that the second product holds it in fp32 as the sum had it. For fp16 the values of
+// each matrix are first scaled by a power of two that brings the row's largest to [2^14, 2^15): one of 2^-15 of that or more
+// keeps its 24 bits, a smaller one is held to 2^-39 of the largest. The matrix's factor comes back with the adapter's scale.
 template <typename T, int RANK16, int CTAS>
 __device__ __forceinline__ void store_row(const Inner<T>& u, int r, const float2 (&v)[RANK16], float scale) {
+    constexpr int RP = RANK16 * 16;
     const int lane = threadIdx.x % 32;
-    float up = 1.0f, down = scale;
+    float up[RANK16];
     if constexpr (std::is_same_v<T, __half>) {
-        float top = 0.0f;
+        float top[RANK16];      // of a lane's columns, then of their matrix: RP / 2 lanes of an i, or two i of all lanes
 #pragma unroll
-        for (int i = 0; i < RANK16; ++i) top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
-        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-        if (top > 1e-30f && top < 1e30f) {
-            const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
-            up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-            down = scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        for (int i = 0; i < RANK16; ++i) top[i] = fmaxf(fabsf(v[i].x), fabsf(v[i].y));
+#pragma unroll
+        for (int i = 0; i < RANK16; ++i) {
+            if (RANK16 == 8 && i % 2 == 0) top[i] = fmaxf(top[i], top[(i + 1) % RANK16]);
+            if (RANK16 == 8 && i % 2) {
+                top[i] = top[i - 1];
+                continue;
+            }
+#pragma unroll
+            for (int k = RP < 64 ? RP / 4 : 16; k; k >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], k));
+        }
+#pragma unroll
+        for (int i = 0; i < RANK16; ++i) {
+            const int c = lane * 2 + i * 64, to = c % RP / 2;
+            const int e = max(static_cast<int>(__float_as_uint(top[i]) >> 23) - 127 - 14, -113);
+            up[i] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            if (c < u.cols && to < CTAS)
+                st_cluster_u32(u.factor + r * 4 + c / RP, to,
+                               __float_as_uint(scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23)));
         }
     }
 #pragma unroll
     for (int i = 0; i < RANK16; ++i) {
         const int c = lane * 2 + i * 64;
         if (c >= u.cols) continue;
-        float a = v[i].x * up, b = v[i].y * up;
+        float a = v[i].x, b = v[i].y;
+        if constexpr (std::is_same_v<T, __half>) a *= up[i], b *= up[i];
 #pragma unroll
         for (int k = 0; k < PARTS<T>; ++k) {
             const uint32_t bits = pack(a, b, T());
@@ -304,7 +319,13 @@ __device__ __forceinline__ void store_row(const Inner<T>& u, int r, const float2
             for (int w = 0; w < CTAS; ++w) st_cluster_u32(u.part + k * u.part_size + r * u.stride + c, w, bits);
         }
     }
-    if (lane < CTAS) st_cluster_u32(u.factor + r, lane, __float_as_uint(down));
+}
+
+// What row r's sums over u of matrix m are multiplied by.
+template <typename T>
+__device__ __forceinline__ float factor_of(const Inner<T>& u, int r, int m, float scale) {
+    if constexpr (std::is_same_v<T, __half>) return u.factor[r * 4 + m];
+    else return scale;
 }
 
 // The fragments of u's steps s and s + 1 of a lane's two rows (g and g + 8 from `u` on).
@@ -481,7 +502,6 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) adapt_few(AdaptParams p) {
     }
     cluster_sync_all();     // (the last access to another CTA's memory was before it)
 
-    const float fa = u.factor[g], fb = u.factor[g + 8];
     for (int b = block_lo + warp; b < block_hi; b += WARPS) {
         const Block block = block_at(p, b);
         const int col = block.col + q * 8;
@@ -499,6 +519,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) adapt_few(AdaptParams p) {
                                                       : zero;
             }
         });
+        const float fa = factor_of(u, g, block.m, scale), fb = factor_of(u, g + 8, block.m, scale);
         if (in && ra >= 0) *reinterpret_cast<uint4*>(out + ra * p.out_stride + col) = added<T>(ya, acc, 0, fa);
         if (in && rb >= 0) *reinterpret_cast<uint4*>(out + rb * p.out_stride + col) = added<T>(yb, acc, 2, fb);
     }
@@ -738,14 +759,12 @@ __global__ void __launch_bounds__(many_warps(RANK16) * 32, RANK16 >= 4 ? 1 : 2) 
     cluster_sync_all();     // (the last access to another CTA's memory was before it)
 
     T* to[F][2];
-    float scale_of[F][2];
 #pragma unroll
     for (int f = 0; f < F; ++f)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int row = la + f * 16 + r * 8, at = tile_rows[row];
             to[f][r] = at >= 0 ? static_cast<T*>(p.out) + at * p.out_stride + q * 8 : nullptr;
-            scale_of[f][r] = u.factor[row];
         }
     const uint32_t y_at = la * 256 + (col_warp * 4 + q ^ (g & 1) << 2) * 16;
     const uint32_t b_at = M * 256 + (col_warp * 32 + g) * ROW * 16;
@@ -806,7 +825,8 @@ __global__ void __launch_bounds__(many_warps(RANK16) * 32, RANK16 >= 4 ? 1 : 2) 
             for (int r = 0; r < 2; ++r)
                 if (to[f][r])
                     *reinterpret_cast<uint4*>(to[f][r] + block.col) =
-                        added<T>(ld_shared_v4(from + y_at + (f * 16 + r * 8) * 256), acc[f], r * 2, scale_of[f][r]);
+                        added<T>(ld_shared_v4(from + y_at + (f * 16 + r * 8) * 256), acc[f], r * 2,
+                                 factor_of(u, la + f * 16 + r * 8, block.m, scale));
     }
     cp_async_wait<0>();
 }
