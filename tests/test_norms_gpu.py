@@ -385,3 +385,24 @@ def test_rows_up_to_the_most_there_may_be(dev):
     assert (buffer[rows] == -1).all()
     with pytest.raises(EspError):
         norms.BlockNorm(8)(x.expand(rows + 1, 8), out=x.expand(rows + 1, 8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,gate_dtype,d", [(torch.float32, torch.float32, 2048), (torch.float32, torch.float32, 515),
+                                                (torch.bfloat16, torch.bfloat16, 2048), (torch.float16, torch.float16, 515),
+                                                (torch.bfloat16, torch.float32, 64), (torch.float32, torch.float32, 8200)])
+@pytest.mark.parametrize("gate", ["channel", "row", "element"])
+@pytest.mark.parametrize("rows", [3, 3001])
+def test_sigmoid_of_an_fp32_stream(dev, dtype, gate_dtype, d, gate, rows):
+    """r = 1 sigmoid(g) in fp32: the exponential is within 2 units, 1 + e and 1 / (1 + e) round once each: 3 units, of 2^-23
+    of the value at most (and their products, far below a hundredth of one)."""
+    if gate != "row" and gate_dtype != dtype:
+        pytest.skip("rows of another type than x: one kernel for all gates")
+    shape = {"channel": (d,), "row": (rows, 1), "element": (rows, d)}[gate]
+    g = (torch.rand(*shape, device=dev, generator=torch.Generator(device=dev).manual_seed(d)) * 107 - 87).to(gate_dtype)
+    one = torch.ones(rows, d, device=dev, dtype=dtype)
+    r, _ = norms.BlockNorm(d, gate_act="sigmoid")(one, torch.zeros(rows, d, device=dev), gate=g)
+    want = torch.sigmoid(g.double()).expand(rows, d)
+    assert r.dtype == torch.float32
+    worst = ((r.double() - want).abs() / want).max().item()
+    assert worst <= 3.03 * 2.0 ** -23, worst * 2 ** 23
