@@ -412,10 +412,11 @@ size_t esp_adapt_ws_bytes(int t_rows, int slots);
  * A temperature that is not above 0 is greedy: d_i stands iff it is the argmax, which replaces it otherwise.
  * tokens int32 [requests][max_drafts + 1] gets the tokens that stand and the drawn one, -1 after them; accepted int32
  * [requests] the number that stand; probs fp32 [requests][max_drafts + 1] p_i of each token (temperature 1 for a greedy
- * request), 0 after them. NaN logits count as -inf (a token ruled out); a row with nothing left gives -1 and ends the
- * request. A drafted id outside [0, vocab) never stands. Drafts past max_drafts are not looked at; a request whose
- * starts do not fit rows and n_drafts gets no token. vocab and max_drafts are at most 2^30. Strides in elements; temperature NULL: 1, and one outside
- * [1e-30, 1e30] counts as the nearer end.
+ * request), 0 after them. NaN logits count as -inf (a token ruled out), a probability below 2^-126 of its row's largest as 0;
+ * a row with nothing left gives -1 and ends the request. A drafted id outside [0, vocab) never stands. Drafts past max_drafts
+ * are not looked at; a request whose starts do not fit rows and n_drafts gets no token. vocab and max_drafts are at most
+ * 2^30. Noise is any number above 0. Strides in elements; temperature NULL: 1, and one outside [1e-30, 1e30] counts as the
+ * nearer end.
  */
 int esp_verify(const void* logits, int dtype, long long stride, long long rows, int vocab, const int* starts,
                int requests, const int* drafts, const float* uniform, long long n_drafts, const void* draft_probs,

@@ -295,3 +295,17 @@ def test_sizes_past_the_calls_integers_are_refused(monkeypatch):
     for vocab, drafts in ((2 ** 31 - 1, 1), (2 ** 30 + 1, 1), (8, 2 ** 31 - 1)):
         assert _lib.lib().esp_verify(16, 1, 8, 2, vocab, 16, 1, 16, 16, 1, None, 2, 8, 16, 8, None, drafts, 16, 16, 16,
                                      None) == _lib.ESP_ERR_INVALID
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [3, 1003, 20000])
+@pytest.mark.parametrize("probs", [None, torch.float32])
+@pytest.mark.parametrize("low,high", [(-149, -126), (-149, 3), (126, 128), (-126, 128)])
+def test_noise_over_the_types_whole_range(dev, V, probs, low, high):
+    """Noise that is subnormal, or whose reciprocal is: still argmax of weight / noise."""
+    kw = batch(dev, [2, 0, 3, 1, 0], V, torch.float32, probs, seed=V, peak=2.0, temperatures=(1.0, 0.7))
+    g = torch.Generator().manual_seed(V)
+    noise = torch.exp2(torch.rand(5, V, generator=g, dtype=torch.float64) * (high - low) + low).clamp(2.0 ** -149, 3.4e38)
+    kw["noise"] = noise.float().to(dev)
+    assert (kw["noise"] > 0).all() and kw["noise"].isfinite().all()
+    run_and_check(**kw)

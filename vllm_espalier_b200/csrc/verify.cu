@@ -361,7 +361,8 @@ struct Best {
     int at = -1;
 };
 
-// The race over [lo, hi) from w: many loads are asked for before the first is used, a thread compares eight scores at
+// The race over [lo, hi) from w, by reciprocals of the noise (one unit of fp32 off, 0 past 2^126, infinite where it is
+// subnormal: see race_exact): many loads are asked for before the first is used, a thread compares eight scores at
 // once and `at` is where its eight consecutive ids start (or a single id). SUBTRACT: a drafted token was turned down and
 // the drafter's probabilities are taken off.
 template <bool SAFE, bool SUBTRACT, typename T, typename Q>
@@ -474,6 +475,40 @@ __device__ __forceinline__ void race_all(Shared& sh, const T* row, const Q* q, c
     }
 }
 
+// The race over row i of request b where its scores leave what rcp() and fp32 hold (noise that is subnormal or past 2^126):
+// the same weights, the quotient in double, brought to where fp32 holds the largest, `top` by reciprocals. Pointers and ids
+// are made anew, so that the kernel need not keep them for it.
+constexpr float SCORE_LO = 0x1p-100f, SCORE_HI = 0x1p100f;
+template <typename T, typename Q>
+__device__ __noinline__ void race_exact(Shared& sh, const VerifyParams& p, int b, int i, Segments own, float m, float c,
+                                        float inv_z, bool safe, float top) {
+    constexpr bool GIVEN = !std::is_same_v<Q, NoProbs>;
+    const long long at = static_cast<long long>(p.starts[b]) + i;
+    const T* row = static_cast<const T*>(p.logits) + (at + b) * p.stride;
+    const float* noise = p.noise + b * p.noise_stride;
+    const bool fell = i < min(p.starts[b + 1] - p.starts[b], p.max_drafts);
+    const int out = fell && !GIVEN ? p.drafts[at] : -1;
+    const Weights wt{m, c, m * c, safe ? inv_z : inv_z * ex2(-fmaf(m, c, -(m * c)))};
+    const double scale = top > 1.0f ? 0x1p-60 : 0x1p180;
+    float best = 0.0f;
+    int id = INT_MAX;
+    for (int v = own.lo(0) + threadIdx.x; v < own.hi(own.count - 1); v += THREADS) {
+        const float l = f32(row[v]), e = safe ? wt.e<true>(l) : wt.e<false>(l);
+        float qv = 0.0f;
+        if constexpr (GIVEN)
+            if (fell) qv = f32(static_cast<const Q*>(p.draft_probs)[at * p.probs_stride + v]);
+        const float s = static_cast<float>(static_cast<double>(fmaf(e, wt.scale, -qv)) / noise[v] * scale);
+        if (v != out && s > best) best = s, id = v;
+    }
+    const float most = warp_max(best);
+    id = __reduce_min_sync(0xffffffffu, best == most ? id : INT_MAX);
+    if ((threadIdx.x & 31) == 0) {
+        const unsigned long long key = id == INT_MAX ? 0 : score_key(most, id);
+        sh.warps[threadIdx.x >> 5] = {__uint_as_float(static_cast<uint32_t>(key >> 32)),
+                                      __uint_as_float(static_cast<uint32_t>(key)), 0, 0};
+    }
+}
+
 struct Split {      // a request's vocabulary over segments and CTAs
     int ctas_log2, segments, own, size;
     bool ahead;
@@ -482,7 +517,7 @@ struct Split {      // a request's vocabulary over segments and CTAs
 // A cluster of CTAs a request, each with its share of the vocabulary's segments: rows in order until a drafted token falls.
 // Every CTA reads the same joined parts and so takes the same decisions.
 template <typename T, typename Q>
-__global__ void __launch_bounds__(THREADS, RESIDENT) verify_kernel(VerifyParams p, Split split) {
+__global__ void __launch_bounds__(THREADS, RESIDENT) verify_kernel(const __grid_constant__ VerifyParams p, Split split) {
     __shared__ Shared sh;
     constexpr bool GIVEN = !std::is_same_v<Q, NoProbs>;
     const int b = blockIdx.x >> split.ctas_log2, ctas = 1 << split.ctas_log2, rank = blockIdx.x & (ctas - 1);
@@ -569,7 +604,12 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) verify_kernel(VerifyParams 
                 if (safe) race_all<true, false>(sh, row, q, noise, out, own, wt);
                 else race_all<false, false>(sh, row, q, noise, out, own, wt);
             }
-            const unsigned long long key = exchange.largest();
+            unsigned long long key = exchange.largest();
+            const float top = __uint_as_float(static_cast<uint32_t>(key >> 32));
+            if (!(top >= SCORE_LO && top <= SCORE_HI)) {
+                race_exact<T, Q>(sh, p, b, n, own, m, c, inv_z, safe, top);
+                key = exchange.largest();
+            }
             token = key_id(key);
             if (!key) {         // no weight left: the target's likeliest token
                 token = careful_part(row, own, c, exchange).at;
