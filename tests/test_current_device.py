@@ -55,3 +55,18 @@ def test_launch_is_on_the_tensors_device(monkeypatch, make, current, device):
     with FakeTensorMode():
         make(torch.device("cuda", device))()
     assert calls == [(device, 1000 + device)] and at == [current]
+
+
+def test_host_tensors_do_not_reach_the_library(monkeypatch):
+    """ext() calls that do not look at their tensors' device themselves: the stream of a device that has none is refused."""
+    calls = []
+    monkeypatch.setattr(_lib, "lib", lambda: types.SimpleNamespace(esp_combine=lambda *a: calls.append(a) or _lib.ESP_OK,
+                                                                   esp_down_combine=lambda *a: calls.append(a) or _lib.ESP_OK))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    t = torch.zeros(4, 8)
+    with pytest.raises(ValueError):
+        _lib._Ext.combine(t, t, t, 1, 8, 4)
+    with pytest.raises(ValueError):
+        _lib._Ext.down_epilogue(t, t, t, t, 1, 4, 8, 1, 4, 4)
+    assert not calls

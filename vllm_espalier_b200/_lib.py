@@ -115,7 +115,10 @@ def check(rc: int):
 
 
 def stream_ptr(device: torch.device | None = None) -> int:
-    """The current stream's handle, without the Stream object torch.cuda.current_stream makes (about 2 us a call)."""
+    """The current stream's handle, without the Stream object torch.cuda.current_stream makes (about 2 us a call). A device
+    without streams is refused as there: for some calls this is what keeps host memory from a kernel."""
+    if device is not None and device.type != "cuda":
+        raise ValueError(f"expected CUDA tensors, got {device}")
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     return torch._C._cuda_getCurrentRawStream(index)
 
