@@ -406,3 +406,12 @@ def test_sigmoid_of_an_fp32_stream(dev, dtype, gate_dtype, d, gate, rows):
     assert r.dtype == torch.float32
     worst = ((r.double() - want).abs() / want).max().item()
     assert worst <= 3.03 * 2.0 ** -23, worst * 2 ** 23
+
+
+def test_weights_that_are_no_tensors_are_refused():
+    """A list or an array is no norm without a weight."""
+    for kw in (dict(pre=[1.0] * 8), dict(post=torch.ones(8).numpy()), dict(pre=2.0), dict(pre=True, pre_bias=[0.0] * 8),
+               dict(post=True, post_bias=True)):
+        with pytest.raises(ValueError, match="tensor"):
+            norms.BlockNorm(8, **kw)
+    assert norms.BlockNorm(8, pre=True, post=False).has_pre and not norms.BlockNorm(8, pre=False).has_pre

@@ -42,6 +42,9 @@ class BlockNorm:
             raise ValueError(f"gate_act {gate_act!r}: expected one of {sorted(ACTS)}")
         on, tensors = {}, {}
         for name, w, b in (("pre", pre, pre_bias), ("post", post, post_bias)):
+            if not (w is None or isinstance(w, (bool, torch.Tensor))) or not (b is None or isinstance(b, torch.Tensor)):
+                raise ValueError(f"{name} must be a tensor, True or None and its bias a tensor or None, got "
+                                 f"{type(w).__name__} and {type(b).__name__}")
             on[name] = w is not None and w is not False
             if b is not None and not on[name]:
                 raise ValueError(f"{name}_bias without the {name} norm")
