@@ -11,10 +11,10 @@
 // tile's size or on the rows beside it.
 //
 // The products are small (rank 16: 35 flops a byte), so bytes bound a large batch and latency a small one. mma.sync and not
-// tcgen05: the tensor pipe is 6 to 17% busy, u is born in registers and goes back into them, and both paths share one order
-// of summation. Measured (q | k | v of 2048 -> 5120, rank 16 unless said): one token 5.8 us (ids, one round trip to A, two
-// cluster barriers, one to B and y), 48 rows of 64 adapters of rank 32 14 us, 8192 rows of 12 prompts 61 us = 3.3 TB/s
-// (52% of a plain copy; plan 4 us, the rest is stage hand-overs), 3001 rows at rank 64 82 us (15%: the parts that hold u in
+// tcgen05: the tensor pipe is 7 to 20% busy, u is born in registers and goes back into them, and both paths share one order
+// of summation. Measured (q | k | v of 2048 -> 5120, bf16, rank 16 unless said): one token 5.9 us (ids, one round trip to A,
+// two cluster barriers, one to B and y), 48 rows of 64 adapters of rank 32 14 us, 8192 rows of 12 prompts 61 us = 3.3 TB/s
+// (52% of a plain copy; plan 4 us, the rest is stage hand-overs), 3001 rows at rank 64 81 us (15%: the parts that hold u in
 // fp32 treble the second product, and sums or parts and the ring leave one CTA an SM).
 #include <cuda_runtime.h>
 
@@ -30,8 +30,8 @@ namespace esp {
 namespace {
 
 constexpr int SEGMENTS = 8, MAX_SLOTS = 4096;
-// Up to this many rows every CTA finds its tile's rows itself, above it a launch of its own does: 17 / 32 / 48 / 64 rows 7.6 /
-// 8.2 / 9.0 / 10.7 us so, 10.1 / 11.1 / 10.9 / 11.1 with the plan.
+// Up to this many rows every CTA finds its tile's rows itself, above it a launch of its own does: 17 / 32 / 48 / 64 rows 8.0 /
+// 8.2 / 9.1 / 10.7 us so, 10.3 / 11.2 / 11.2 / 11.4 with the plan.
 constexpr int NO_PLAN = 64;
 
 struct AdaptParams {
@@ -528,8 +528,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) adapt_few(AdaptParams p) {
 // ---------------------------------------------------------------------------------------------------------------
 // Many rows an adapter (prefill): tiles of 64 rows, CTAS a cluster; four shares of the columns by two groups of 32 rows
 // (eight warps of two fragments, two CTAs an SM) or, from rank 33 on, where shared memory leaves one CTA an SM, by four
-// groups of 16 (8192 x rank 16: 57 us against 64 with four groups; x rank 32: 97 against 95, but 69 against 80 with one
-// matrix; 3001 x rank 64: 73 against 76 with two). One ring of shared memory carries both products: stages of 64 k of x and
+// groups of 16 (8192 x rank 16: 60 us against 72 with four groups, x rank 32 93 against 112; 3001 x rank 64: 80 against 83
+// with two). One ring of shared memory carries both products: stages of 64 k of x and
 // A, then stages of 128 columns of y and B, filled by 16-byte asynchronous copies, so that the second product's operands are
 // on their way while the sums are joined. Rows of a stage are 128 bytes or more apart and their 16-byte pieces swapped by
 // halves on odd rows (piece ^ 4), so that a quarter load (two rows, four pieces) meets every bank once.
@@ -898,9 +898,11 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
     const bool half = ad->dtype == F16;
     const int parts = half ? PARTS<__half> : PARTS<__nv_bfloat16>;
     // Tiles of 64 rows where the inner columns fit a CTA, tiles of 16 need more than two rounds of the GPU's clusters, and
-    // adapters have enough rows each that tiles of 64 are not mostly empty. Measured, 16 / 64 rows a tile, us, rank 16, 32 and
-    // 64: 512 rows 15 / 17, 18 / 23, 22 / 24; 1024 rows 21 / 20, 26 / 27, 34 / 39; 1536 rows 30 / 21, 37 / 28, 49 / 39. 64
-    // adapters mixed row by row: 1536 rows 41 / 32, 51 / 47, 67 / 100; 3000 rows 66 / 37, 80 / 55, 102 / 104.
+    // there are enough rows a slot that tiles of 64 are not mostly empty if every slot is in use (which ids occur is not known
+    // here: with 12 of 512 slots in use, 8192 rows of rank 16 take 156 us for it, and 61 with 12 of 16). Measured, 16 / 64 rows
+    // a tile, us, rank 16, 32 and 64, four prompts: 512 rows 15 / 19, 18 / 26, 23 / 27; 1024 rows 22 / 21, 27 / 29, 36 / 42;
+    // 1536 rows 30 / 22, 39 / 29, 51 / 42. 64 adapters mixed row by row: 1536 rows 41 / 34, 53 / 48, 70 / 111; 3000 rows
+    // 67 / 38, 82 / 53, 106 / 114.
     const int clusters = std::max(device_sms() / 18, 1) * (18 * 2 / FEW_CTAS);
     const bool many = t_rows > 2 * FEW_ROWS * clusters && t_rows / ad->slots >= (steps >= 4 ? 40 : 24) && cols <= MANY_COLS;
     const int m = many ? MANY_ROWS : FEW_ROWS;
@@ -924,7 +926,8 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
     }
     // CTAs a tile: what takes the least rounds x (a CTA's share of a tile + what it spends on joining sums). Places: two CTAs
     // an SM (one from rank 33 on, or where a ring of two stages does not fit twice), as many whole clusters as the 18 SMs of a
-    // GPC hold. Measured: 128 tiles of rank 16 with 2 / 4 / 8 CTAs 68 / 74 / 90 us, 47 tiles of rank 64 with 4 / 8 75 / 85 us.
+    // GPC hold. Measured: 8192 rows of rank 16 with 2 / 4 / 8 CTAs 60 / 65 / 83 us, of rank 32 124 / 93 / 111, 3001 of rank
+    // 64 with 4 / 8 80 / 95 us.
     const int half_sm = HALF_SM, tiles = (t_rows + m - 1) / m + std::min(ad->slots, t_rows / m) / 2;
     int ctas = 8;       // (fits whatever fits at all)
     double best = 1e30;
@@ -935,7 +938,7 @@ extern "C" int esp_adapt(const esp_adapters_t* ad, const void* x, long long x_st
         const double work = ((tiles * c + places - 1) / places) * (1.0 / c + CTA_COST);
         if (work < best) best = work, ctas = c;
     }
-    // Two stages where that leaves an SM to two CTAs: q | k | v at rank 32, 8192 rows 97 us against 125 with three and one CTA.
+    // Two stages where that leaves an SM to two CTAs: q | k | v at rank 32, 8192 rows 93 us against 127 with three and one CTA.
     const bool three = steps != 2 || many_bytes(cols, steps, 3, ctas, parts) <= half_sm;
     const int least = three || many_bytes(cols, steps, 2, ctas, parts) > half_sm ? 3 : 2;
     const int room = steps < 4 && many_bytes(cols, steps, least, ctas, parts) <= half_sm ? half_sm : MAX_SMEM;
