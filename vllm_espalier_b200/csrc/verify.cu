@@ -37,6 +37,8 @@ __device__ __forceinline__ float f32(float v) { return v; }
 __device__ __forceinline__ float f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+// 2^x to two units of fp32, 0 below 2^-126. Sums are fp32's own; a call's probabilities come out within 4e-7 of the 64-bit ones
+// (relative, over the cases of the operators' benchmark; an fp32 softmax by exact exponentials and divisions: 2e-7).
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
